@@ -67,7 +67,8 @@ def _quantise(w, group):
     n, k = w.shape
     parts = w.view(n, k // group, group)
     low, high = parts.amin(2), parts.amax(2)
-    scale, offset = ((high - low) / 15).to(torch.bfloat16), low.to(torch.bfloat16)
+    fifteen = torch.full((1, 1), 15, dtype=w.dtype, device=w.device)   # (a number instead would be multiplied by as 1 / 15)
+    scale, offset = ((high - low) / fifteen).to(torch.bfloat16), low.to(torch.bfloat16)
     s, b = scale.float()[:, :, None], offset.float()[:, :, None]
     q = torch.where(s > 0, (parts - b) / s, torch.zeros_like(parts)).round_().clamp_(0, 15)
     return q.view(n, k).to(torch.int32), scale, offset
@@ -191,11 +192,11 @@ def exact(case, seed):
     n, k, group = case["n"], case["k"], case["group"]
     if case["op"] == "quantise":
         w = state["w"].double()
-        out = torch.empty_like(w)
+        out, steps = torch.empty_like(w), torch.full((n, 1), 15, dtype=torch.float64, device="cuda")
         for at in range(0, k, group):
             part = w[:, at:at + group]
             low, high = part.min(1, keepdim=True).values, part.max(1, keepdim=True).values
-            s, b = ((high - low) / 15).to(torch.bfloat16).double(), low.to(torch.bfloat16).double()
+            s, b = ((high - low) / steps).to(torch.bfloat16).double(), low.to(torch.bfloat16).double()
             q = torch.nan_to_num((part - b) / s, nan=0.0).round().clamp(0, 15)
             out[:, at:at + group] = (q * s + b).to(torch.bfloat16).double()
         return out
