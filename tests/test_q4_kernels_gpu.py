@@ -1,0 +1,248 @@
+"""Matrices in four bits: making them, taking them back, and the products with them, against the format written out in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+import q4_helpers as q4
+from velox_b200.csrc import ops
+
+pytestmark = pytest.mark.gpu
+
+
+def made(n, k, group, seed, dtype=torch.bfloat16):
+    """(a matrix in four bits, what it stands for in 64 bits)"""
+    g = torch.Generator().manual_seed(seed)
+    w = (torch.randn(n, k, generator=g) * 0.02 * (0.5 + torch.rand(n, 1, generator=g))).to(dtype).cuda()
+    m = ops.quantize_q4(w, group)
+    return m, q4.matrix(*q4.unpack(m), group)
+
+
+def rows_of(m, k, seed):
+    g = torch.Generator().manual_seed(1000 + seed)
+    x = torch.randn(m, k, generator=g)
+    x[:, ::97] *= 8
+    x = x.to(torch.bfloat16)
+    return x.cuda(), x.to(torch.float64).numpy()
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,k", [(1, 128), (15, 384), (16, 1), (17, 5), (200, 1024)])
+def test_quantize(n, k, group, dtype):
+    k = k if k > 8 else k * group   # (an odd number of groups too)
+    w = torch.randn(n, k, generator=torch.Generator().manual_seed(n + k)).mul_(0.02).to(dtype)
+    m = ops.quantize_q4(w.cuda(), group)
+    q, s, b = q4.quantise(w.float().numpy(), group)
+    for got, want in zip(q4.unpack(m), (q, s, b)):
+        assert np.array_equal(got, want)
+    assert np.array_equal(ops.dequantize_q4(m).double().cpu().numpy(), q4.matrix(q, s, b, group))
+    # within half a scale (and the scale's, the offset's and the value's roundings) of what was given
+    limit = np.repeat(s, group, 1) * (0.5 + 15 * q4.HALF_BF16) + 2 * q4.HALF_BF16 * np.abs(np.repeat(b, group, 1)) + q4.HALF_BF16 * w.double().abs().numpy()
+    assert (np.abs(q4.matrix(q, s, b, group) - w.double().numpy()) <= limit).all()
+
+
+def test_padding_is_zero():
+    m = ops.quantize_q4(torch.full((17, 96), 3.0, dtype=torch.bfloat16, device="cuda"), 32)
+    codes, affine = m.codes, m.affine
+    assert codes.shape == (2, 2, 4, 8, 2, 2) and affine.shape == (2, 4, 8, 2, 2)
+    assert int(codes[1, :, :, 1:].abs().sum()) == 0 and float(affine[1, :, 1:].abs().sum()) == 0
+    assert int(codes[:, 1, 2:].abs().sum()) == 0 and float(affine[:, 3].abs().sum()) == 0
+    assert float(affine[1, :, 0, 1].abs().sum()) == 0
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_groups_at_the_edges_of_the_format(group):
+    """Constant groups, zeros, tiny and huge values, ties, infinities and NaN: each in a group of its own, its neighbours untouched."""
+    g = np.zeros((16, group), np.float32)
+    g[0] = 0.37
+    g[2] = np.linspace(0, 15, group)                     # scale 1, offset 0: codes with ties
+    g[3] = np.where(np.arange(group) % 2, 0.5, 15.0)
+    g[3, 0] = 0.0
+    g[4] = 1e-39 * np.arange(group)
+    g[5] = 3e38
+    g[5, 1] = -3e38                                      # a range beyond float32
+    g[6] = 1e38 * np.sin(np.arange(group))
+    g[7, 3] = np.nan
+    g[8, 1] = np.inf
+    g[9, 2] = -np.inf
+    g[10] = -5.0
+    g[10, 7] = -4.0
+    g[11] = 1.0
+    g[11, 5] = 1.0 + 2.0 ** -7
+    w = np.concatenate([g, np.roll(g, 1, 0), g[::-1]], 1)
+    m = ops.quantize_q4(torch.from_numpy(w).cuda(), group)
+    want = q4.quantise(w, group)
+    for got, x in zip(q4.unpack(m), want):
+        assert np.array_equal(got, x, equal_nan=True)
+    assert np.isnan(want[1][7, 0]) and np.isnan(want[1][5, 0]) and not np.isnan(want[1][6, 0])
+    assert np.array_equal(ops.dequantize_q4(m).double().cpu().numpy(), q4.matrix(*want, group), equal_nan=True)
+
+
+def test_quantize_rows_of_a_wider_matrix():
+    w = torch.randn(33, 512, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).cuda()
+    m = ops.quantize_q4(w[:, 64:320], 64)
+    for got, want in zip(q4.unpack(m), q4.quantise(w[:, 64:320].float().cpu().numpy(), 64)):
+        assert np.array_equal(got, want)
+
+
+SIZES = [(1, 16, 64, 64), (1, 2048, 2048, 64), (2, 1, 32, 32), (3, 17, 96, 32), (5, 1000, 1056, 32), (8, 4096, 128, 128), (7, 40, 5120, 128),
+         (8, 333, 4096, 64), (9, 100, 256, 64), (16, 130, 1024, 128), (17, 250, 2080, 32), (33, 129, 640, 64), (64, 512, 512, 64),
+         (65, 1003, 1056, 32), (127, 256, 1984, 64), (128, 128, 4224, 128), (129, 200, 320, 64), (200, 2048, 2048, 64), (257, 144, 384, 128),
+         (300, 15, 96, 32), (513, 700, 704, 64), (1025, 272, 256, 64)]
+
+
+@pytest.mark.parametrize("m,n,k,group", SIZES)
+@pytest.mark.parametrize("out_dtype,biased", [(torch.bfloat16, False), (torch.float32, True)])
+def test_product(m, n, k, group, out_dtype, biased):
+    w, w64 = made(n, k, group, m + n)
+    x, x64 = rows_of(m, k, n)
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(5)).cuda() if biased else None
+    got = ops.gemm_q4(x, w, bias, out_dtype)
+    want = x64 @ w64.T + (bias.double().cpu().numpy() if biased else 0)
+    assert got.dtype == out_dtype
+    q4.close(got, want, q4.sum_bound(x64, w64) + (2.0 ** -23 * np.abs(want) if biased else 0), out_dtype)
+    ops.check_device_errors()
+
+
+@pytest.mark.parametrize("m,n,k,group", SIZES)
+def test_gated(m, n, k, group):
+    (gate, g64), (up, u64) = made(n, k, group, m), made(n, k, group, n + 7)
+    x, x64 = rows_of(m, k, n + 1)
+    name = sorted(ops.ACTIVATIONS)[(m + n) % len(ops.ACTIVATIONS)]
+    got = ops.gated_q4(x, gate, up, name)
+    want, bound = q4.gated(x64, g64, u64, name)
+    q4.close(got, want, bound, torch.bfloat16)
+    ops.check_device_errors()
+
+
+@pytest.mark.parametrize("name", sorted(ops.ACTIVATIONS))
+@pytest.mark.parametrize("m", [4, 40])
+def test_every_activation(m, name):
+    (gate, g64), (up, u64) = made(96, 256, 64, 1), made(96, 256, 64, 2)
+    x, x64 = rows_of(m, 256, 3)
+    x, x64 = x * 8, x64 * 8
+    want, bound = q4.gated(x64, g64, u64, name)
+    q4.close(ops.gated_q4(x, gate, up, name), want, bound, torch.bfloat16)
+
+
+def test_product_is_that_of_the_dense_matrix():
+    """The same matrix, dense and in four bits, through the engine's products: float32 sums of the same terms."""
+    w, w64 = made(256, 512, 64, 9)
+    x, x64 = rows_of(8, 512, 9)
+    dense = ops.gemm_bf16(x, ops.dequantize_q4(w), None, torch.float32).double().cpu().numpy()
+    got = ops.gemm_q4(x, w, None, torch.float32).double().cpu().numpy()
+    assert (np.abs(dense - got) <= 2 * q4.sum_bound(x64, w64)).all()
+
+
+def test_a_rows_result_does_not_depend_on_its_neighbours():
+    w, _ = made(300, 1024, 64, 4)
+    up, _ = made(300, 1024, 64, 5)
+    x, _ = rows_of(8, 1024, 4)
+    whole, pair = ops.gemm_q4(x, w), ops.gated_q4(x, w, up)
+    for m in range(1, 8):
+        assert torch.equal(ops.gemm_q4(x[:m], w), whole[:m])
+        assert torch.equal(ops.gated_q4(x[m:], w, up), pair[m:])
+
+
+@pytest.mark.parametrize("m", [4, 70, 300])
+def test_the_same_result_every_time(m):
+    w, _ = made(512, 2048, 64, 4)
+    x, _ = rows_of(m, 2048, 4)
+    first = ops.gemm_q4(x, w, None, torch.float32)
+    for _ in range(5):
+        assert torch.equal(ops.gemm_q4(x, w, None, torch.float32, w_ready=True), first)
+
+
+@pytest.mark.parametrize("m", [6, 50, 150])
+def test_values_that_are_not_finite_stay_in_their_rows(m):
+    w, w64 = made(64, 256, 64, 4)
+    x, x64 = rows_of(m, 256, 4)
+    x[1, 5] = float("nan")
+    x[3, 200] = float("inf")
+    got = ops.gemm_q4(x, w, None, torch.float32)
+    good = [i for i in range(m) if i not in (1, 3)]
+    q4.close(got[good], (x64 @ w64.T)[good], q4.sum_bound(x64[good], w64), torch.float32)
+    assert bool(got[1].isnan().all()) and not bool(got[3].isfinite().any())
+    # a group of W that stands for NaN: its row of W, that column of the result
+    dense = torch.randn(64, 256, generator=torch.Generator().manual_seed(8)).to(torch.bfloat16).cuda()
+    dense[7, 9] = float("inf")
+    bad = ops.gemm_q4(rows_of(m, 256, 5)[0], ops.quantize_q4(dense, 64), None, torch.float32)
+    assert bool(bad[:, 7].isnan().all()) and bool(bad[:, :7].isfinite().all()) and bool(bad[:, 8:].isfinite().all())
+
+
+@pytest.mark.parametrize("m", [0, 1, 5, 40, 150])
+def test_rows_of_a_wider_tensor_and_none(m):
+    w, w64 = made(100, 320, 64, 6)
+    wide, _ = rows_of(max(m, 2), 400, 6)
+    x = wide[:m, 8:328]
+    got = ops.gemm_q4(x, w, None, torch.float32)
+    x64 = x.double().cpu().numpy()
+    q4.close(got, x64 @ w64.T, q4.sum_bound(x64, w64), torch.float32)
+    assert ops.gated_q4(x, w, w).shape == (m, 100)
+    if m == 1:   # (a lone row's stride says nothing)
+        assert torch.equal(ops.gemm_q4(x.as_strided((1, 320), (3, 1)), w, None, torch.float32), got)
+
+
+@pytest.mark.parametrize("m", [3, 90])
+def test_on_another_stream_and_in_a_graph(m):
+    w, _ = made(256, 512, 64, 7)
+    up, _ = made(256, 512, 64, 8)
+    x, _ = rows_of(m, 512, 7)
+    y, _ = rows_of(m, 512, 70)
+    want = [(ops.gemm_q4(v, w, None, torch.float32), ops.gated_q4(v, w, up)) for v in (x, y)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = ops.gemm_q4(x, w, None, torch.float32), ops.gated_q4(x, w, up)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got[0], want[0][0]) and torch.equal(got[1], want[0][1])
+    fed = x.clone()
+    graphs = []
+    for _ in range(2):   # (two captures share nothing)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            h = ops.gated_q4(fed, w, up, w_ready=True)
+            out = ops.gemm_q4(fed, w, None, torch.float32, w_ready=True), h
+        graphs.append((graph, out))
+    for v, (a, b) in ((y, want[1]), (x, want[0])):
+        fed.copy_(v)
+        for graph, out in graphs:
+            graph.replay()
+        for graph, out in graphs:
+            assert torch.equal(out[0], a) and torch.equal(out[1], b)
+    ops.check_device_errors()
+
+
+@pytest.mark.parametrize("m", [2, 70])
+def test_a_matrix_made_just_before(m):
+    """Without `w_ready` nothing of the matrix is read before the kernel that makes it has ended."""
+    x, x64 = rows_of(m, 1024, 1)
+    for seed in range(20):
+        dense = torch.randn(640, 1024, device="cuda").to(torch.bfloat16)
+        w = ops.quantize_q4(dense, 64)
+        got = ops.gemm_q4(x, w, None, torch.float32)
+        w64 = q4.matrix(*q4.unpack(w), 64)
+        q4.close(got, x64 @ w64.T, q4.sum_bound(x64, w64), torch.float32)
+
+
+def test_refusals():
+    w, _ = made(32, 128, 64, 1)
+    x, _ = rows_of(2, 128, 1)
+    for call, why in [
+            (lambda: ops.gemm_q4(x.float(), w), "bfloat16 a"), (lambda: ops.gemm_q4(x[:, :64], w), "bfloat16 a"),
+            (lambda: ops.gemm_q4(x[0], w), "bfloat16 a"), (lambda: ops.gemm_q4(x, w, None, torch.float16), "bfloat16 or float32 out"),
+            (lambda: ops.gemm_q4(rows_of(2, 132, 1)[0][:, :128], w), "16-byte aligned"),
+            (lambda: ops.gemm_q4(rows_of(2, 136, 1)[0][:, 1:129], w), "16-byte aligned"),
+            (lambda: ops.gemm_q4(rows_of(128, 2, 1)[0].t(), w), "contiguous"),
+            (lambda: ops.gemm_q4(x[:1].expand(3, 128), w), "contiguous"),
+            (lambda: ops.gemm_q4(x, w, torch.zeros(31, device="cuda")), "bias"),
+            (lambda: ops.gemm_q4(x, w, torch.zeros(32, device="cuda", dtype=torch.bfloat16)), "bias"),
+            (lambda: ops.gemm_q4(x, w, torch.zeros(64, device="cuda")[::2]), "bias"),
+            (lambda: ops.gemm_q4(x.cpu(), w), "CUDA tensors"),
+            (lambda: ops.gated_q4(x, w, w, "swish"), "unknown activation"),
+            (lambda: ops.gated_q4(x, w, made(33, 128, 64, 1)[0]), "one shape"), (lambda: ops.gated_q4(x, w, made(32, 128, 32, 1)[0]), "one shape"),
+            (lambda: ops.quantize_q4(x.half(), 64), "bfloat16 or float32"), (lambda: ops.quantize_q4(x, 48), "groups of"),
+            (lambda: ops.quantize_q4(x[:, :96], 64), "multiple of the group"), (lambda: ops.quantize_q4(x[:0], 64), "positive"),
+            (lambda: ops.quantize_q4(x[:, 1:65], 64), "aligned"), (lambda: ops.quantize_q4(x.t(), 64), "contiguous")]:
+        with pytest.raises(ops.KernelError, match=why):
+            call()

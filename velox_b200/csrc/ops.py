@@ -194,6 +194,9 @@ def _declare(lib) -> None:
         "vx_moe_gemm_capped": [P, I, P, I, P, P, P, I, P, I, I, I, I, I, I, I, I, I, P, F, F, P],
         "vx_moe_gemm_tcgen05_capped": [P, P, P, I, I, I, I, I, I, I, I, P, P, I, P, P, P, I, F, F, P],
         "vx_latent_gather_window": [P, P, I, P, P, P, P, I, P, I, I, I, I, I, I, I, P],
+        "vx_quantize_q4": [P, P, P, I, I, c_longlong, I, I, P],
+        "vx_dequantize_q4": [P, P, P, I, I, I, P],
+        "vx_gemm_q4": [P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, P],
     }
     lib.vx_set_pdl_mask.argtypes = [I]
     lib.vx_host_word.argtypes, lib.vx_host_word.restype = [], c_void_p
@@ -1961,6 +1964,120 @@ def gemm_bf16(a: torch.Tensor, w: torch.Tensor, bias=None, out_dtype: Optional[t
         _check(library().vx_add_bias(_ptr(summed), _ptr(bias), _ptr(out), summed.shape[0], summed.shape[1],
                                      dtype_code(out_dtype), 1.0, _stream()), "add_bias")
     return out
+
+
+Q4_GROUPS = (32, 64, 128)   # neighbours along a row that share a scale and an offset
+
+
+class Q4Matrix:
+    """A matrix [rows, depth] held in four bits: `codes` and `affine` (scales and offsets) as `csrc/q4.cuh` lays them out, groups of
+    `group` neighbours of a row.  Element (n, k) stands for bfloat16(q s + b), its code q and its group's bfloat16 scale s and offset b.
+    Made by `quantize_q4`, or from tensors of that layout: codes int32 [ceil(rows / 16), ceil(depth / 64), 4, 8, 2, 2], affine
+    bfloat16 [ceil(rows / 16), groups, 8, 2, 2], both contiguous."""
+    __slots__ = ("codes", "affine", "rows", "depth", "group")
+
+    def __init__(self, codes: torch.Tensor, affine: torch.Tensor, rows: int, depth: int, group: int):
+        tiles, blocks, groups = _q4_sizes(rows, depth, group)
+        _need(codes.dtype == torch.int32 and tuple(codes.shape) == (tiles, blocks, 4, 8, 2, 2) and codes.is_contiguous(),
+              "Q4Matrix: codes must be contiguous int32 %s for [%d, %d]" % ((tiles, blocks, 4, 8, 2, 2), rows, depth))
+        _need(affine.dtype == torch.bfloat16 and tuple(affine.shape) == (tiles, groups, 8, 2, 2) and affine.is_contiguous(),
+              "Q4Matrix: scales and offsets must be contiguous bfloat16 %s for [%d, %d] in groups of %d" % ((tiles, groups, 8, 2, 2), rows, depth, group))
+        _need(codes.device == affine.device, "Q4Matrix: codes on %s, scales and offsets on %s" % (codes.device, affine.device))
+        _need(codes.data_ptr() % 16 == 0 and affine.data_ptr() % 16 == 0, "Q4Matrix: 16-byte aligned tensors")
+        self.codes, self.affine, self.rows, self.depth, self.group = codes, affine, int(rows), int(depth), int(group)
+
+    @property
+    def shape(self) -> Tuple[int, int]:
+        return self.rows, self.depth
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() * 4 + self.affine.numel() * 2
+
+
+def _q4_sizes(rows: int, depth: int, group: int) -> Tuple[int, int, int]:
+    """(row tiles of 16, blocks of 64 k, groups) of a matrix in four bits."""
+    _need(group in Q4_GROUPS, "four-bit matrices have groups of %s, not %r" % (Q4_GROUPS, group))
+    _need(0 < rows < 1 << 31 and 0 < depth < 1 << 31 and depth % group == 0,
+          "a four-bit matrix [%s, %s]: rows and depth positive, the depth a multiple of the group %d" % (rows, depth, group))
+    blocks = -(-depth // 64)
+    return -(-rows // 16), blocks, blocks * 64 // group
+
+
+def _elsewhere(t: torch.Tensor) -> bool:
+    """True for a tensor of another CUDA device than the current one."""
+    return t.is_cuda and t.device.index != (_GET_DEVICE() if _GET_DEVICE is not None else torch.cuda.current_device())
+
+
+def quantize_q4(w: torch.Tensor, group: int = 64) -> Q4Matrix:
+    """`w` [N, K] (bfloat16 or float32, rows 16-byte aligned, K a multiple of `group`) in four bits: per group of neighbours
+    s = bfloat16((max - min) / 15), b = bfloat16(min), q = round((w - b) / s) within 0 to 15 (ties to even; s = 0: q = 0).  A group with a value
+    that is not finite, or whose scale is not, stands for NaN."""
+    _dev(w)
+    _need(w.dim() == 2 and w.dtype in (torch.bfloat16, torch.float32) and w.stride(1) == 1, "quantize_q4: bfloat16 or float32 w [N, K], rows contiguous")
+    n, k = w.shape
+    tiles, blocks, groups = _q4_sizes(n, k, group)
+    if _elsewhere(w):
+        with torch.cuda.device(w.device):
+            return quantize_q4(w, group)
+    codes = torch.empty((tiles, blocks, 4, 8, 2, 2), dtype=torch.int32, device=w.device)
+    affine = torch.empty((tiles, groups, 8, 2, 2), dtype=torch.bfloat16, device=w.device)
+    _check(library().vx_quantize_q4(_ptr(w), _ptr(codes), _ptr(affine), n, k, w.stride(0) if n > 1 else k, group, dtype_code(w.dtype), _stream()),
+           "quantize_q4")
+    return Q4Matrix(codes, affine, n, k, group)
+
+
+def dequantize_q4(w: Q4Matrix) -> torch.Tensor:
+    """The bfloat16 matrix that `w` stands for: what the products multiply with."""
+    _dev(w.codes, w.affine)
+    if _elsewhere(w.codes):
+        with torch.cuda.device(w.device):
+            return dequantize_q4(w)
+    out = torch.empty(w.shape, dtype=torch.bfloat16, device=w.device)
+    _check(library().vx_dequantize_q4(_ptr(w.codes), _ptr(w.affine), _ptr(out), w.rows, w.depth, w.group, _stream()), "dequantize_q4")
+    return out
+
+
+def _q4_product(what: str, a: torch.Tensor, w: Q4Matrix, up: Optional[Q4Matrix], bias, out_dtype, act: int, w_ready: bool) -> torch.Tensor:
+    _dev(a, w.codes, w.affine, bias)
+    _need(a.dtype == torch.bfloat16 and a.dim() == 2 and a.shape[1] == w.depth, "%s: bfloat16 a [M, %d]" % (what, w.depth))
+    m, k = a.shape
+    lda = a.stride(0) if m > 1 else k
+    _need((a.stride(1) == 1 and lda % 8 == 0 and lda >= k and a.data_ptr() % 16 == 0) or m == 0, "%s: rows of a contiguous and 16-byte aligned" % what)
+    _need(out_dtype in (torch.bfloat16, torch.float32), "%s: bfloat16 or float32 out, not %s" % (what, out_dtype))
+    _need(a.device == w.device and (bias is None or bias.device == a.device), "%s: all tensors on one device" % what)
+    if bias is not None:
+        _need(bias.dtype == torch.float32 and bias.numel() == w.rows and bias.is_contiguous(), "%s: float32 bias of N elements" % what)
+    if _elsewhere(a):
+        with torch.cuda.device(a.device):
+            return _q4_product(what, a, w, up, bias, out_dtype, act, w_ready)
+    out = torch.empty((m, w.rows), dtype=out_dtype, device=a.device)
+    if m == 0:
+        return out
+    _check(library().vx_gemm_q4(_ptr(a), _ptr(w.codes), _ptr(w.affine), _ptr(up.codes) if up else None, _ptr(up.affine) if up else None, _ptr(bias),
+                                _ptr(out), m, w.rows, k, lda, w.rows, w.group, act, dtype_code(out_dtype), 1 if w_ready else 0, _stream()), what)
+    return out
+
+
+def gemm_q4(a: torch.Tensor, w: Q4Matrix, bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+            w_ready: bool = False) -> torch.Tensor:
+    """a [M, K] (bfloat16) times the matrix that `w` [N, K] stands for, transposed (+ float32 `bias` [N]); float32 sums, rounded once to
+    `out_dtype` (bfloat16 or float32).  `w_ready`: see `gemm_nt_simt`."""
+    return _q4_product("gemm_q4", a, w, None, bias, out_dtype or torch.bfloat16, 0, w_ready)
+
+
+def gated_q4(a: torch.Tensor, gate: Q4Matrix, up: Q4Matrix, activation: str = "silu", w_ready: bool = False) -> torch.Tensor:
+    """act(a Wg^T) * (a Wu^T) in one kernel, [M, N] bfloat16: both projections of a gated feed-forward with matrices in four bits of one
+    shape and group; activation and product on the float32 sums, rounded once.  `w_ready`: see `gemm_nt_simt`."""
+    _need(activation in ACTIVATIONS, "gated_q4: unknown activation %r" % (activation,))
+    _need(gate.shape == up.shape and gate.group == up.group and gate.device == up.device,
+          "gated_q4: gate %s and up %s of one shape, group and device" % (gate.shape, up.shape))
+    return _q4_product("gated_q4", a, gate, up, None, torch.bfloat16, ACTIVATIONS[activation], w_ready)
+
 
 
 def sample(logits: torch.Tensor, temperature=None, top_p=None, uniform=None) -> torch.Tensor:

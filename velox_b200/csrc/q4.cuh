@@ -1,0 +1,32 @@
+// Matrices held in four bits: the layout, and codes to the bfloat16 values that they stand for.
+//
+// A row's K is cut into groups of 32, 64 or 128 neighbours.  A group keeps a bfloat16 scale s and offset b, its elements a code q from 0
+// to 15, and an element is W = bfloat16(q s + b): q s + b is rounded once, so every kernel multiplies with the same matrix, whatever the
+// number of rows.  (A scale has 8 significant bits and a code 4, so W would need 12 and more to be exact.  The rounding moves W by at most
+// half a step, 2^-9 of it; the code has moved it by up to half a scale, some 2^-5 of a group's largest element.)
+//
+// Codes: blocks of 16 rows by 64 k, 512 bytes, along K first: [N / 16][K / 64][t 4][r 8][half 2][word 2] of 32 bits; row 16 i + 8 half + r,
+// k = 64 c + 16 t + 8 word + 2 p + e in bits 4 (4 e + p).
+//   - A lane 4 r + t of mma.sync.m16n8k16 has rows r and r + 8 on its side: its 32 codes of a block are 16 neighbouring bytes.
+//   - A thread that owns a row (a lane of tensor memory) takes four times 8 bytes, and the threads of 16 rows 128 neighbouring ones.
+//   - `(word >> 4 p) & 0x000f000f` is a pair of neighbouring k, the lower one in the lower half.
+// Scales and offsets: [N / 16][groups][r 8][half 2] pairs (s in the lower half of 32 bits, b in the upper), groups = K / group with K rounded
+// up to 64.  Rows and k beyond the matrix have codes, scales and offsets of 0, so they stand for 0.
+#pragma once
+#include "common.cuh"
+
+#define Q4_BLOCK_WORDS 128   // 32-bit words of a block of 16 rows by 64 k
+
+// Both halves of a register: the scale, the offset.
+__device__ __forceinline__ unsigned q4_scale(unsigned affine) { return __byte_perm(affine, 0, 0x1010); }
+__device__ __forceinline__ unsigned q4_offset(unsigned affine) { return __byte_perm(affine, 0, 0x3232); }
+// Eight codes to four pairs of bfloat16.  A code in the lower bits of 128.0 (0x4300) is 128 + q exactly; less 128 exactly q; the
+// multiply-add rounds once.
+__device__ __forceinline__ void q4_values(unsigned word, unsigned scale, unsigned offset, unsigned (&w)[4]) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        unsigned v = ((word >> (4 * p)) & 0x000f000fu) | 0x43004300u;
+        asm("sub.rn.bf16x2 %0, %1, %2;\n" : "=r"(v) : "r"(v), "r"(0x43004300u));
+        asm("fma.rn.bf16x2 %0, %1, %2, %3;\n" : "=r"(w[p]) : "r"(v), "r"(scale), "r"(offset));
+    }
+}
