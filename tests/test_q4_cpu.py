@@ -40,7 +40,7 @@ def test_the_entry_points_refuse_before_they_launch():
     A = 1 << 20
 
     def product(x=A, codes=A, affine=A, codes1=None, affine1=None, bias=None, out=A, m=2, n=32, k=128, ldx=128, ldo=32, group=64, act=0, dtype=1):
-        return lib.vx_gemm_q4(x, codes, affine, codes1, affine1, bias, out, m, n, k, ldx, ldo, group, act, dtype, 0, None)
+        return lib.vx_gemm_q4(x, codes, affine, codes1, affine1, bias, out, m, n, k, ldx, ldo, group, act, dtype, 0, A, None)
     assert product(m=0) == 0 and product(n=0) == 0
     for change, code in [(dict(k=0), SHAPE), (dict(k=96), SHAPE), (dict(group=16), SHAPE), (dict(ldx=120), SHAPE), (dict(ldo=31), SHAPE),
                          (dict(codes1=A), SHAPE), (dict(codes1=A, affine1=A, bias=A), SHAPE), (dict(codes1=A, affine1=A, act=6), SHAPE),

@@ -128,15 +128,21 @@ static int q4_launch(const bf16* x, const Q4Pair& w, const float* bias, TO* out,
     return VX_OK;
 }
 
+extern "C" int vx_gemm_q4_tc(const void* x, const void* codes, const void* affine, const void* codes1, const void* affine1, const float* bias,
+                             void* out, int M, int N, int K, int ldx, int ldo, int group, int act, int out_dtype, int w_ready, int* error,
+                             cudaStream_t stream);
+
 // One matrix (codes1 null), or gate (codes, affine) and up (codes1, affine1): out = act(gate) * up.  N rows each.  `w_ready`: the
 // matrices are nothing that the kernel launched just before this one writes.
 extern "C" int vx_gemm_q4(const void* x, const void* codes, const void* affine, const void* codes1, const void* affine1, const float* bias,
                           void* out, int M, int N, int K, int ldx, int ldo, int group, int act, int out_dtype, int w_ready,
-                          cudaStream_t stream) {
+                          int* error, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return VX_OK;
     if (K <= 0 || (group != 32 && group != 64 && group != 128) || K % group || ldx < K || ldo < N) return VX_ERR_SHAPE;
     if (codes1 && (!affine1 || bias || act < 0 || act > VX_ACT_LAST)) return VX_ERR_SHAPE;
     if (ldx & 7 || (((uintptr_t)x) | ((uintptr_t)codes) | ((uintptr_t)affine) | ((uintptr_t)codes1) | ((uintptr_t)affine1)) & 15) return VX_ERR_ALIGN;
+    if (M > 8)
+        return vx_gemm_q4_tc(x, codes, affine, codes1, affine1, bias, out, M, N, K, ldx, ldo, group, act, out_dtype, w_ready, error, stream);
     const Q4Pair w = {{(const unsigned*)codes, (const unsigned*)codes1}, {(const unsigned*)affine, (const unsigned*)affine1}};
 #define Q4_CALL(G, T) q4_launch<G, T>((const bf16*)x, w, bias, (T*)out, M, N, K, ldx, ldo, act, group, w_ready, stream)
     if (out_dtype == VX_BF16) return codes1 ? Q4_CALL(true, bf16) : Q4_CALL(false, bf16);

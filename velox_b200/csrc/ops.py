@@ -196,7 +196,8 @@ def _declare(lib) -> None:
         "vx_latent_gather_window": [P, P, I, P, P, P, P, I, P, I, I, I, I, I, I, I, P],
         "vx_quantize_q4": [P, P, P, I, I, c_longlong, I, I, P],
         "vx_dequantize_q4": [P, P, P, I, I, I, P],
-        "vx_gemm_q4": [P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, P],
+        "vx_gemm_q4": [P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, P, P],
+        "vx_gemm_q4_tc_shape": [P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, P, P],
     }
     lib.vx_set_pdl_mask.argtypes = [I]
     lib.vx_host_word.argtypes, lib.vx_host_word.restype = [], c_void_p
@@ -1967,6 +1968,7 @@ def gemm_bf16(a: torch.Tensor, w: torch.Tensor, bias=None, out_dtype: Optional[t
 
 
 Q4_GROUPS = (32, 64, 128)   # neighbours along a row that share a scale and an offset
+Q4_FEW_ROWS = 8             # rows up to which the products stream the matrix through mma.sync; above they have bounded waits
 
 
 class Q4Matrix:
@@ -2059,7 +2061,9 @@ def _q4_product(what: str, a: torch.Tensor, w: Q4Matrix, up: Optional[Q4Matrix],
     if m == 0:
         return out
     _check(library().vx_gemm_q4(_ptr(a), _ptr(w.codes), _ptr(w.affine), _ptr(up.codes) if up else None, _ptr(up.affine) if up else None, _ptr(bias),
-                                _ptr(out), m, w.rows, k, lda, w.rows, w.group, act, dtype_code(out_dtype), 1 if w_ready else 0, _stream()), what)
+                                _ptr(out), m, w.rows, k, lda, w.rows, w.group, act, dtype_code(out_dtype), 1 if w_ready else 0, _error_address(a.device), _stream()), what)
+    if m > Q4_FEW_ROWS:
+        note_bounded_wait()
     return out
 
 
