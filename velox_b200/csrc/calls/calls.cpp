@@ -11,6 +11,7 @@
 // points' addresses.
 #include <Python.h>
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/Dtype.h>
@@ -30,6 +31,9 @@ struct Entries {
     int (*gemm_turned)(P, P, void*, int, int, int, int, int, int, int, int, int, int, void*, void*);
     int (*prefill)(P, int, int, P, P, int, P, int, P, P, P, void*, int, float, int, int, int, int, int, int, int, void*, int, void*, void*);
     int (*decode)(P, int, P, P, P, int, P, P, P, void*, int, void*, int, float, int, int, int, int, int, int, int, int, int, void*);
+    int (*quantize_q4)(P, void*, void*, int, int, long long, int, int, void*);
+    int (*dequantize_q4)(P, P, void*, int, int, int, void*);
+    int (*gemm_q4)(P, P, P, P, P, P, void*, int, int, int, int, int, int, int, int, int, void*, void*);
 } entry;
 
 const int DTYPE_F32 = 0, DTYPE_BF16 = 1;   // the library's codes
@@ -316,6 +320,82 @@ PyObject* decode_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// A matrix in four bits: its codes, its scales and offsets, its sizes.
+struct Q4 {
+    Arg codes, affine;
+    Q4(PyObject* c, PyObject* a) : codes(c), affine(a) {}
+    static int64_t blocks(int64_t depth) { return (depth + 63) / 64; }
+    static bool sized(int rows, int depth, int group) {
+        return rows > 0 && depth > 0 && (group == 32 || group == 64 || group == 128) && depth % group == 0;
+    }
+    bool fine(int rows, int depth, int group, int device) const {
+        const int64_t tiles = ((int64_t)rows + 15) / 16;
+        return is(codes, at::kInt) && is16(affine) && codes->is_contiguous() && affine->is_contiguous() && aligned16(*codes) && aligned16(*affine) &&
+               codes->numel() == tiles * blocks(depth) * 128 && affine->numel() == tiles * (blocks(depth) * 64 / group) * 32 &&
+               codes->get_device() == device && affine->get_device() == device;
+    }
+};
+
+// (a, codes, affine, up's codes or None, up's affine or None, bias, rows, depth, group, activation, out dtype, w is ready, the error word's address)
+PyObject* gemm_q4(PyObject*, PyObject* const* o, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 13) NOT_HERE;
+    Arg a(o[0]);
+    Q4 w(o[1], o[2]), up(o[3], o[4]);
+    Optional bias(o[5]);
+    Scalars sc;
+    const int N = sc.i(o[6]), K = sc.i(o[7]), group = sc.i(o[8]), act = sc.i(o[9]), ready = sc.i(o[11]);
+    void* const error = sc.p(o[12]);
+    const bool gated = o[3] != Py_None;
+    if (sc.bad || !is16(a) || !THPDtype_Check(o[10]) || !bias.is(at::kFloat) || !Q4::sized(N, K, group)) NOT_HERE;
+    const int device = c10::cuda::current_device();
+    const at::ScalarType kind = ((THPDtype*)o[10])->scalar_type;
+    if (code_of(kind) < 0 || a->dim() != 2 || a->size(1) != K || a->size(0) <= 0 || !small(a->size(0)) || a->get_device() != device || !w.fine(N, K, group, device) ||
+        (gated && !up.fine(N, K, group, device)) || (bias && (bias.a->numel() != N || !bias.a->is_contiguous() || bias.a->get_device() != device)))
+        NOT_HERE;
+    const int64_t M = a->size(0), lda = M > 1 ? a->stride(0) : K;
+    if (a->stride(1) != 1 || lda % 8 || lda < K || !small(lda) || !aligned16(*a)) NOT_HERE;
+    at::Tensor out = fresh(M, N, kind, *a);
+    LAUNCH(rc, entry.gemm_q4(a->data_ptr(), w.codes->data_ptr(), w.affine->data_ptr(), gated ? up.codes->data_ptr() : nullptr,
+                             gated ? up.affine->data_ptr() : nullptr, bias.ptr(), out.data_ptr(), (int)M, N, K, (int)lda, N, group, act,
+                             code_of(kind), ready, error, s));
+    return result(rc, std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// (w, group): (codes, affine)
+PyObject* quantize_q4(PyObject*, PyObject* const* o, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 2) NOT_HERE;
+    Arg w(o[0]);
+    Scalars sc;
+    const int group = sc.i(o[1]);
+    if (sc.bad || !w || w->dim() != 2 || !small(w->size(0)) || !small(w->size(1)) || !Q4::sized((int)w->size(0), (int)w->size(1), group)) NOT_HERE;
+    const int64_t N = w->size(0), K = w->size(1), ldw = N > 1 ? w->stride(0) : K, tiles = (N + 15) / 16, blocks = Q4::blocks(K);
+    if (code_of(w->scalar_type()) < 0 || w->stride(1) != 1 || w->get_device() != c10::cuda::current_device()) NOT_HERE;
+    at::Tensor codes = at::empty({tiles, blocks, 4, 8, 2, 2}, w->options().dtype(at::kInt));
+    at::Tensor affine = at::empty({tiles, blocks * 64 / group, 8, 2, 2}, w->options().dtype(at::kBFloat16));
+    LAUNCH(rc, entry.quantize_q4(w->data_ptr(), codes.data_ptr(), affine.data_ptr(), (int)N, (int)K, (long long)ldw, group,
+                                 code_of(w->scalar_type()), s));
+    if (rc) return PyLong_FromLong(rc);
+    return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(codes)), THPVariable_Wrap(std::move(affine)));
+    END_HANDLE_TH_ERRORS
+}
+
+// (codes, affine, rows, depth, group)
+PyObject* dequantize_q4(PyObject*, PyObject* const* o, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 5) NOT_HERE;
+    Q4 w(o[0], o[1]);
+    Scalars sc;
+    const int N = sc.i(o[2]), K = sc.i(o[3]), group = sc.i(o[4]);
+    if (sc.bad || !Q4::sized(N, K, group) || !w.fine(N, K, group, c10::cuda::current_device())) NOT_HERE;
+    at::Tensor out = fresh(N, K, at::kBFloat16, *w.codes);
+    LAUNCH(rc, entry.dequantize_q4(w.codes->data_ptr(), w.affine->data_ptr(), out.data_ptr(), N, K, group, s));
+    return result(rc, std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
 // (path of the kernel library): looks the entry points up; once, before any other call
 PyObject* bind(PyObject*, PyObject* arg) {
     const char* path = PyUnicode_AsUTF8(arg);
@@ -332,6 +412,9 @@ PyObject* bind(PyObject*, PyObject* arg) {
         {"vx_gemm_turned", (void**)&entry.gemm_turned},
         {"vx_paged_prefill_attention_tc", (void**)&entry.prefill},
         {"vx_paged_decode_attention_shape", (void**)&entry.decode},
+        {"vx_quantize_q4", (void**)&entry.quantize_q4},
+        {"vx_dequantize_q4", (void**)&entry.dequantize_q4},
+        {"vx_gemm_q4", (void**)&entry.gemm_q4},
     };
     for (const auto& w : wanted) {
         *w.at = dlsym(lib, w.name);
@@ -343,6 +426,7 @@ PyObject* bind(PyObject*, PyObject* arg) {
 #define FAST(f) {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {{"bind", bind, METH_O, nullptr}, FAST(add_rmsnorm), FAST(qk_norm_rope_kv), FAST(gated_act), FAST(gemm_bf16),
                          FAST(gemm_tcgen05), FAST(gemm_turned), FAST(tcgen05_supported), FAST(prefill_attention), FAST(decode_attention),
+                         FAST(gemm_q4), FAST(quantize_q4), FAST(dequantize_q4),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "velox_b200_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

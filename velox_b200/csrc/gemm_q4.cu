@@ -9,124 +9,242 @@
 // order: the same result on every run, and a row's result does not depend on the rows beside it.
 #include "q4.cuh"
 
-__device__ __forceinline__ uint4 q4_stream16(const unsigned* p) {
+__device__ __forceinline__ unsigned q4_smem(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void q4_copy16(unsigned to, const char* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ uint4 q4_lds16(unsigned at) {
     uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
     return v;
 }
-__device__ __forceinline__ uint2 q4_stream8(const unsigned* p) {
+__device__ __forceinline__ uint2 q4_lds8(unsigned at) {
     uint2 v;
-    asm volatile("ld.global.nc.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ uint4 q4_x16(const bf16* p) {
+    uint4 v;
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
 }
 __device__ __forceinline__ void q4_mma(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 struct Q4Pair { const unsigned *codes[2], *affine[2]; };   // the matrix, or gate and up
 
-template <bool GATED, typename TO, int WARPS, int UNROLL>
-__global__ void __launch_bounds__(WARPS * 32)
+// What a block forms at a time: 16 rows of W; 32 rows (two tiles, for which x is read once); 16 gate rows and their up rows.
+enum { Q4_ONE = 0, Q4_TWO = 1, Q4_GATED = 2 };
+// A warp's step: BLOCKS code blocks, neighbours along K, with their scales and offsets; of both tiles where there are two.
+template <int FORM, int GROUP, int BLOCKS> struct Q4Step {
+    static constexpr int mats = FORM == Q4_ONE ? 1 : 2, codes = BLOCKS * 512, affine = BLOCKS * 64 * 64 / GROUP, bytes = codes + affine;
+};
+
+template <int FORM, typename TO, int GROUP, int NT, int WARPS, int BLOCKS, int DEPTH, int PER_SM>
+__global__ void __launch_bounds__(WARPS * 32, PER_SM)
 gemm_q4_kernel(const bf16* __restrict__ x, const Q4Pair w, const float* __restrict__ bias, TO* __restrict__ out, int M, int N, int K, int ldx,
-               int ldo, int act, int blocks, int groups, int group_shift, int w_ready) {
-    constexpr int MATS = GATED ? 2 : 1;
-    __shared__ float red[MATS][WARPS][16][9];
+               int ldo, int act, int blocks, int units, int w_ready) {
+    typedef Q4Step<FORM, GROUP, BLOCKS> Step;
+    constexpr bool GATED = FORM == Q4_GATED, TWO = FORM == Q4_TWO, BOTH = FORM != Q4_ONE;
+    static_assert(BLOCKS * 64 % GROUP == 0, "a step holds whole groups");
+    constexpr int MATS = Step::mats, SLOT = MATS * Step::bytes;
+    extern __shared__ __align__(16) unsigned char q4_ring[];
+    __shared__ float red[2][MATS][WARPS][16][8 * NT + 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
-    const size_t tile = blockIdx.x;
-    const int m0 = blockIdx.y * 8;
-    const unsigned *codes[MATS], *affine[MATS];
-#pragma unroll
-    for (int i = 0; i < MATS; ++i) {
-        codes[i] = w.codes[i] + tile * blocks * Q4_BLOCK_WORDS + (t * 8 + r) * 4;
-        affine[i] = w.affine[i] + tile * groups * 16 + r * 2;
-    }
-    float acc[MATS][4] = {};
-    uint4 q[MATS][UNROLL];
-    uint2 a[MATS][UNROLL];
-    int c = warp;
-    auto ask = [&]() {
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const int cu = c + u * WARPS;
-            if (cu < blocks) {
-#pragma unroll
-                for (int i = 0; i < MATS; ++i) {
-                    q[i][u] = q4_stream16(codes[i] + (size_t)cu * Q4_BLOCK_WORDS);
-                    a[i][u] = q4_stream8(affine[i] + ((cu * 64 + t * 16) >> group_shift) * 16);
-                }
-            }
+    // the warp's code blocks of a tile: neighbours, as many for every warp as there can be (whole groups)
+    constexpr int UNIT = GROUP == 128 ? 2 : 1;
+    const int lo = warp * (blocks / UNIT) / WARPS * UNIT, mine = (warp + 1) * (blocks / UNIT) / WARPS * UNIT - lo;
+    const int my_tiles = mine > 0 ? (units - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x : 0;
+    const size_t tile_codes = (size_t)blocks * (Q4_BLOCK_WORDS * 4), tile_affine = (size_t)blocks * (64 * 64) / GROUP;
+    const size_t unit_codes = tile_codes << TWO, unit_affine = tile_affine << TWO;
+    const unsigned ring = q4_smem(q4_ring) + warp * (DEPTH * SLOT);
+    // what is asked for next
+    const char* ask_q = reinterpret_cast<const char*>(w.codes[0]) + blockIdx.x * unit_codes + (size_t)lo * 512 + lane * 16;
+    const char* ask_a = reinterpret_cast<const char*>(w.affine[0]) + blockIdx.x * unit_affine + (size_t)lo * (64 * 64) / GROUP + lane * 16;
+    // from a tile to its second: the up matrix's, or the next (of the matrix's last there may be none: then the first again, not written)
+    ptrdiff_t up_q, up_a;
+    const int tiles_of_w = (N + 15) / 16;
+    auto second_of = [&](int unit) {
+        if (GATED) {
+            up_q = reinterpret_cast<const char*>(w.codes[1]) - reinterpret_cast<const char*>(w.codes[0]);
+            up_a = reinterpret_cast<const char*>(w.affine[1]) - reinterpret_cast<const char*>(w.affine[0]);
+        } else if (TWO) {
+            const bool there = 2 * unit + 1 < tiles_of_w;
+            up_q = there ? tile_codes : 0;
+            up_a = there ? tile_affine : 0;
         }
     };
-    if (w_ready) ask();
+    int ask_unit = blockIdx.x;
+    second_of(ask_unit);
+    int ask_left = mine, ask_tiles = my_tiles;
+    unsigned ask_at = ring + lane * 16;
+    auto ask = [&]() {
+        if (ask_tiles > 0) {
+#pragma unroll
+            for (int b = 0; b < BLOCKS; ++b)
+                if (b < ask_left) {
+                    q4_copy16(ask_at + b * 512, ask_q + b * 512);
+                    if (BOTH) q4_copy16(ask_at + Step::bytes + b * 512, ask_q + up_q + b * 512);
+                }
+            if (lane * 16 < min(BLOCKS, ask_left) * (64 * 64 / GROUP)) {
+                q4_copy16(ask_at + Step::codes, ask_a);
+                if (BOTH) q4_copy16(ask_at + Step::bytes + Step::codes, ask_a + up_a);
+            }
+            ask_q += Step::codes;
+            ask_a += Step::affine;
+            ask_left -= BLOCKS;
+            if (ask_left <= 0) {   // on to the next tile
+                const int steps = (mine + BLOCKS - 1) / BLOCKS;
+                ask_q += gridDim.x * unit_codes - (size_t)steps * Step::codes;
+                ask_a += gridDim.x * unit_affine - (size_t)steps * Step::affine;
+                ask_left = mine;
+                --ask_tiles;
+                if (TWO) second_of(ask_unit += gridDim.x);
+            }
+        }
+        asm volatile("cp.async.commit_group;\n" ::: "memory");
+        ask_at = ask_at == ring + lane * 16 + (DEPTH - 1) * SLOT ? ring + lane * 16 : ask_at + SLOT;
+    };
+    if (w_ready)
+#pragma unroll 1
+        for (int d = 0; d < DEPTH; ++d) ask();
     pdl_wait();
     pdl_trigger();
-    if (!w_ready) ask();
-    const bool xok = m0 + r < M;
-    const bf16* xr = x + (size_t)(xok ? m0 + r : 0) * ldx + t * 16;
-    while (c < blocks) {
-        uint4 xv[UNROLL][2];
+    if (!w_ready)
+#pragma unroll 1
+        for (int d = 0; d < DEPTH; ++d) ask();
+    // Rows of x beyond the last are the last again: what comes of them is not written.
+    const bf16* xr[NT];
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const int k = (c + u * WARPS) * 64;
-            const bool ok = xok && k + t * 16 < K;
+    for (int j = 0; j < NT; ++j) xr[j] = x + (size_t)min(r + 8 * j, M - 1) * ldx + lo * 64 + t * 16;
+    const bool cut = (K & 63) && lo + mine == blocks;   // the warp's last block reaches beyond K: x counts as 0 there (K is a multiple of the group)
+    const unsigned own = (t * 8 + r) * 16, own_affine = Step::codes + r * 8 + (GROUP == 32 ? (t >> 1) * 64 : 0);
+    unsigned at = ring;
+    const int block_tiles = (units - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+    for (int ti = 0; ti < block_tiles; ++ti) {
+        float acc[MATS][NT][4] = {};
+#pragma unroll 1
+        for (int left = mine; left > 0; left -= BLOCKS) {
+            asm volatile("cp.async.wait_group %0;\n" ::"n"(DEPTH - 1) : "memory");
+            __syncwarp();
+            auto block = [&](int b) {
+                uint4 xv[NT][2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) xv[u][i] = ok ? *reinterpret_cast<const uint4*>(xr + k + 8 * i) : make_uint4(0, 0, 0, 0);
-        }
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            if (c + u * WARPS < blocks) {
+                for (int j = 0; j < NT; ++j) {
+                    if (GROUP == 32 && cut && b == left - 1 && t >= 2) {
+                        xv[j][0] = xv[j][1] = make_uint4(0u, 0u, 0u, 0u);
+                    } else {
+                        xv[j][0] = q4_x16(xr[j] + b * 64);
+                        xv[j][1] = q4_x16(xr[j] + b * 64 + 8);
+                    }
+                }
 #pragma unroll
                 for (int i = 0; i < MATS; ++i) {
-                    const unsigned s0 = q4_scale(a[i][u].x), b0 = q4_offset(a[i][u].x), s1 = q4_scale(a[i][u].y), b1 = q4_offset(a[i][u].y);
+                    const uint4 q = q4_lds16(at + own + i * Step::bytes + b * 512);
+                    const uint2 a = q4_lds8(at + own_affine + i * Step::bytes + (GROUP == 128 ? (b >> 1) * 64 : b * (64 * 64 / GROUP)));
+                    const unsigned s0 = q4_scale(a.x), b0 = q4_offset(a.x), s1 = q4_scale(a.y), b1 = q4_offset(a.y);
 #pragma unroll
                     for (int word = 0; word < 2; ++word) {
                         unsigned w0[4], w1[4];
-                        q4_values(word ? q[i][u].y : q[i][u].x, s0, b0, w0);
-                        q4_values(word ? q[i][u].w : q[i][u].z, s1, b1, w1);
-                        q4_mma(acc[i], w0[0], w1[0], w0[1], w1[1], xv[u][word].x, xv[u][word].y);
-                        q4_mma(acc[i], w0[2], w1[2], w0[3], w1[3], xv[u][word].z, xv[u][word].w);
+                        q4_values(word ? q.y : q.x, s0, b0, w0);
+                        q4_values(word ? q.w : q.z, s1, b1, w1);
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) {
+                            q4_mma(acc[i][j], w0[0], w1[0], w0[1], w1[1], xv[j][word].x, xv[j][word].y);
+                            q4_mma(acc[i][j], w0[2], w1[2], w0[3], w1[3], xv[j][word].z, xv[j][word].w);
+                        }
                     }
                 }
+            };
+            // (A whole step has no branches between its blocks, whose loads can then go ahead of the products before.)
+            if (left >= BLOCKS) {
+#pragma unroll
+                for (int b = 0; b < BLOCKS; ++b) block(b);
+            } else {
+#pragma unroll
+                for (int b = 0; b < BLOCKS - 1; ++b)
+                    if (b < left) block(b);
+            }
+            __syncwarp();   // (the lanes' copies below overwrite what all of them have read)
+            ask();
+            at = at == ring + (DEPTH - 1) * SLOT ? ring : at + SLOT;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) xr[j] += BLOCKS * 64;
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) xr[j] -= (mine + BLOCKS - 1) / BLOCKS * (BLOCKS * 64);
+        // a lane holds out^T[row r (0, 1) and r + 8 (2, 3)][rows 2 t, 2 t + 1 of x]
+        const int buf = ti & 1;
+#pragma unroll
+        for (int i = 0; i < MATS; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int m = 8 * n + 2 * t + (j & 1);
+                    if (m < M) red[buf][i][warp][r + 8 * (j >> 1)][m] = acc[i][n][j];
+                }
+        __syncthreads();   // (the sums that are read here are overwritten after the next of these)
+        const int unit = blockIdx.x + ti * gridDim.x;
+        constexpr int ROWS = TWO ? 32 : 16;
+        for (int e = threadIdx.x; e < ROWS * M; e += WARPS * 32) {
+            const int row = e % ROWS, m = e / ROWS, n = unit * ROWS + row;
+            if (n < N) {
+                float v = 0.f, up = 0.f;
+#pragma unroll
+                for (int i = 0; i < WARPS; ++i) {
+                    v += red[buf][TWO ? row >> 4 : 0][i][row & 15][m];
+                    if (GATED) up += red[buf][MATS - 1][i][row][m];
+                }
+                if (bias) v += bias[n];
+                out[(size_t)m * ldo + n] = from_f32<TO>(GATED ? activation(v, act) * up : v);
             }
         }
-        c += UNROLL * WARPS;
-        ask();
     }
-    // a lane holds out^T[row r (0, 1) and r + 8 (2, 3)][rows 2 t, 2 t + 1 of x]
-#pragma unroll
-    for (int i = 0; i < MATS; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) red[i][warp][r + 8 * (j >> 1)][2 * t + (j & 1)] = acc[i][j];
-    __syncthreads();
-    if (threadIdx.x < 128) {
-        const int row = threadIdx.x & 15, m = threadIdx.x >> 4;
-        const size_t n = tile * 16 + row;
-        if (m0 + m < M && n < (size_t)N) {
-            float v = 0.f, up = 0.f;
-#pragma unroll
-            for (int i = 0; i < WARPS; ++i) {
-                v += red[0][i][row][m];
-                if (GATED) up += red[MATS - 1][i][row][m];
-            }
-            if (bias) v += bias[n];
-            out[(size_t)(m0 + m) * ldo + n] = from_f32<TO>(GATED ? activation(v, act) * up : v);
-        }
-    }
+    asm volatile("cp.async.wait_all;\n" ::: "memory");
 }
 
-template <bool GATED, typename TO>
-static int q4_launch(const bf16* x, const Q4Pair& w, const float* bias, TO* out, int M, int N, int K, int ldx, int ldo, int act, int group,
-                     int w_ready, cudaStream_t stream) {
-    const int blocks = (K + 63) / 64, groups = blocks * 64 / group, shift = group == 32 ? 5 : (group == 64 ? 6 : 7);
-    const long long chunks = (M + 7LL) / 8;
-    if (chunks > 65535) return VX_ERR_LIMIT;
-    VX_LAUNCH_K(VX_K_GEMM, (gemm_q4_kernel<GATED, TO, 8, 4>), dim3((unsigned)((N + 15) / 16), (unsigned)chunks), 256, 0, stream, x, w, bias, out, M, N,
-                K, ldx, ldo, act, blocks, groups, shift, w_ready);
+static int q4_sms() {
+    static int sms[VX_MAX_DEVICES];
+    return vx_sm_count(sms);
+}
+
+template <int FORM, typename TO, int GROUP, int NT, int WARPS, int BLOCKS, int DEPTH, int PER_SM>
+static int q4_go(const bf16* x, const Q4Pair& w, const float* bias, TO* out, int M, int N, int K, int ldx, int ldo, int act, int w_ready,
+                 cudaStream_t stream) {
+    typedef Q4Step<FORM, GROUP, BLOCKS> Step;
+    const int blocks = (K + 63) / 64, rows = FORM == Q4_TWO ? 32 : 16, units = (N + rows - 1) / rows, room = q4_sms() * PER_SM;
+    const size_t smem = (size_t)WARPS * DEPTH * Step::mats * Step::bytes;
+    auto kernel = gemm_q4_kernel<FORM, TO, GROUP, NT, WARPS, BLOCKS, DEPTH, PER_SM>;
+    static bool configured[VX_MAX_DEVICES];
+    if (int rc = vx_configure_smem(kernel, smem, configured)) return rc;
+    VX_LAUNCH_K(VX_K_GEMM, kernel, (unsigned)(units < room ? units : room), WARPS * 32, smem, stream, x, w, bias, out, M, N, K, ldx, ldo, act, blocks,
+                units, w_ready);
     VX_LAUNCH_CHECK();
     return VX_OK;
 }
+
+template <bool GATED, typename TO, int GROUP, int NT>
+static int q4_launch(const bf16* x, const Q4Pair& w, const float* bias, TO* out, int M, int N, int K, int ldx, int ldo, int act,
+                     int w_ready, cudaStream_t stream) {
+    const int tiles = (N + 15) / 16, sms = q4_sms();
+#define Q4_GO(F_, W_, P_) return q4_go<F_, TO, GROUP, NT, W_, 4, 2, P_>(x, w, bias, out, M, N, K, ldx, ldo, act, w_ready, stream)
+    if constexpr (GATED) {
+        if (tiles > 6 * sms) Q4_GO(Q4_GATED, 4, 4);
+        Q4_GO(Q4_GATED, 8, 2);
+    } else {
+        if (tiles <= 2 * sms) Q4_GO(Q4_ONE, 8, 2);
+        if (tiles <= 3 * sms) Q4_GO(Q4_ONE, 8, 3);
+        if (tiles <= 16 * sms) Q4_GO(Q4_TWO, 8, 2);
+        Q4_GO(Q4_TWO, 4, 4);
+    }
+#undef Q4_GO
+}
+
+#define Q4_FEW_ROWS 16
 
 extern "C" int vx_gemm_q4_tc(const void* x, const void* codes, const void* affine, const void* codes1, const void* affine1, const float* bias,
                              void* out, int M, int N, int K, int ldx, int ldo, int group, int act, int out_dtype, int w_ready, int* error,
@@ -141,12 +259,16 @@ extern "C" int vx_gemm_q4(const void* x, const void* codes, const void* affine, 
     if (K <= 0 || (group != 32 && group != 64 && group != 128) || K % group || ldx < K || ldo < N) return VX_ERR_SHAPE;
     if (codes1 && (!affine1 || bias || act < 0 || act > VX_ACT_LAST)) return VX_ERR_SHAPE;
     if (ldx & 7 || (((uintptr_t)x) | ((uintptr_t)codes) | ((uintptr_t)affine) | ((uintptr_t)codes1) | ((uintptr_t)affine1)) & 15) return VX_ERR_ALIGN;
-    if (M > 8)
+    if (M > Q4_FEW_ROWS)
         return vx_gemm_q4_tc(x, codes, affine, codes1, affine1, bias, out, M, N, K, ldx, ldo, group, act, out_dtype, w_ready, error, stream);
     const Q4Pair w = {{(const unsigned*)codes, (const unsigned*)codes1}, {(const unsigned*)affine, (const unsigned*)affine1}};
-#define Q4_CALL(G, T) q4_launch<G, T>((const bf16*)x, w, bias, (T*)out, M, N, K, ldx, ldo, act, group, w_ready, stream)
+#define Q4_ROWS(G, T, GR, NT) q4_launch<G, T, GR, NT>((const bf16*)x, w, bias, (T*)out, M, N, K, ldx, ldo, act, w_ready, stream)
+#define Q4_GROUP(G, T, GR) (M <= 8 ? Q4_ROWS(G, T, GR, 1) : Q4_ROWS(G, T, GR, 2))
+#define Q4_CALL(G, T) (group == 32 ? Q4_GROUP(G, T, 32) : (group == 64 ? Q4_GROUP(G, T, 64) : Q4_GROUP(G, T, 128)))
     if (out_dtype == VX_BF16) return codes1 ? Q4_CALL(true, bf16) : Q4_CALL(false, bf16);
     if (out_dtype == VX_F32) return codes1 ? VX_ERR_DTYPE : Q4_CALL(false, float);
 #undef Q4_CALL
+#undef Q4_GROUP
+#undef Q4_ROWS
     return VX_ERR_DTYPE;
 }

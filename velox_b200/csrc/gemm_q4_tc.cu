@@ -2,17 +2,17 @@
 // out[M,N] = x[M,K] W^T (+ bias), and out[M,N] = act(x Wg^T) * (x Wu^T).
 //
 // The operands are turned, out^T = W x^T: 128 rows of W on the M side of tcgen05.mma, n rows of x as its columns.  W is the instruction's A
-// operand, and A may lie in tensor memory: a lane is a row, a column two neighbouring k.  So a thread makes its own row's 64 k of a
-// step from 32 bytes of codes in registers and stores them with one tcgen05.st; W as bfloat16 exists in tensor memory only.
+// operand, and A may lie in tensor memory: a lane is a row, a column two neighbouring k.  So a thread makes 64 k of its own row
+// from 32 bytes of codes in registers and stores them with one tcgen05.st; W as bfloat16 exists in tensor memory only.
 // Gated, gate and up rows of a feature are the same lane's in two accumulators, and the epilogue joins them without an exchange.
 //
 // Warps of a block:
-//   warp 0       producer: x (128-byte swizzle), codes, scales and offsets of 64 k a stage by TMA; W's first stages are asked for before the
+//   warp 0       producer: x (128-byte swizzle), codes, scales and offsets of a step of 128 k by TMA; W's first stages are asked for before the
 //                wait for the kernel launched before this one (if the caller says that W is ready);
 //   warp 1       tensor memory; issues the products;
-//   warps 2-9    two groups of four that make W's values, step by step in turn (gated: one makes gate, the other up), into eight places in
-//                tensor memory;
-//   warps 10-17  epilogue.
+//   warps 2-17   four groups of four that make W's values, half a step each: two groups every other step, gated two gate and two up of every
+//                step; into places for four steps (gated two) in tensor memory;
+//   warps 18-25  epilogue.
 // K may be cut into `splits` runs, one to each block of a cluster, whose float32 sums are added in ascending order through distributed
 // shared memory: the same result on every run.
 // Every wait on an mbarrier is bounded; a block whose wait runs out records a code in the caller's error word and writes NaN, the other roles run
@@ -23,26 +23,29 @@
 #include "q4.cuh"
 #include "tcgen05_pair.cuh"
 
-#define QT_THREADS 576
-#define QT_MAKERS 2          // first warp of those that make W's values
-#define QT_EPILOGUE 10       // ... and of the epilogue's
-#define QT_PLACES 8          // places for 64 k of W's values in tensor memory, 32 columns each, behind the accumulators
-#define QT_PLACES_AT 256
-#define QT_MAX_STAGES 12
-#define QT_CODES 4096        // bytes of a stage: codes of 128 rows by 64 k
-#define QT_AFFINE 1024       // ... room for their scales and offsets (512, or 1024 for groups of 32)
+#define QT_TEAMS 4           // groups of four warps that make W's values
+#define QT_MAKERS 2          // their first warp
+#define QT_EPILOGUE (QT_MAKERS + 4 * QT_TEAMS)   // ... and the epilogue's
+#define QT_THREADS (32 * (QT_EPILOGUE + 8))
+#define QT_K 128             // k of a step
+#define QT_PLACES_AT 256     // W's values in tensor memory: 256 columns behind the accumulators
+#define QT_MAX_STAGES 8
+#define QT_ROOM (224 * 1024) // shared memory for stages
+#define QT_CODES 8192        // bytes of a stage: codes of 128 rows by 128 k
+#define QT_AFFINE 2048       // ... room for their scales and offsets (512, 1024, 2048 for groups of 128, 64, 32)
 #define QT_ERR_PRODUCER 10
 #define QT_ERR_MMA 11
 #define QT_ERR_EPILOGUE 12
 #define QT_ERR_VALUES 13
 
 struct QtShape {
-    int n;         // rows of x in a tile
-    int splits;    // runs of k
-    int kbs;       // steps of 64 k of a run
+    int n;             // rows of x in a tile
+    int splits;        // runs of k
+    int steps;         // steps of a run
+    int full_w, n2;    // W tiles from full_w on take tiles of n2 rows of x (full_w: all of them, where none do)
     int stages;
 };
-struct QtMaps { CUtensorMap x, codes[2], affine[2]; };
+struct QtMaps { CUtensorMap x, x2, codes[2], affine[2]; };
 
 __device__ __forceinline__ void qt_st32(unsigned taddr, const unsigned (&r)[32]) {
     asm volatile(
@@ -53,7 +56,6 @@ __device__ __forceinline__ void qt_st32(unsigned taddr, const unsigned (&r)[32])
         "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
         "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
-    asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
 }
 __device__ __forceinline__ void qt_ld16(unsigned taddr, unsigned (&r)[16]) {
     asm volatile(
@@ -62,6 +64,8 @@ __device__ __forceinline__ void qt_ld16(unsigned taddr, unsigned (&r)[16]) {
           "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr) : "memory");
 }
+// (What is waited for takes microseconds; this many polls take a good part of a second at least.)
+__device__ __forceinline__ bool qt_wait(unsigned bar, unsigned parity) { return tc_warp_wait(bar, parity, 1 << 20); }
 __device__ __forceinline__ uint2 qt_lds8(unsigned addr) {
     uint2 v;
     asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
@@ -80,8 +84,15 @@ __device__ __forceinline__ float qt_ld_cluster(unsigned addr) {
 __device__ __forceinline__ void qt_arrive(unsigned bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
 }
+// z / (1 + exp(-z)) by the hardware's 2^x and 1 / x (a few 2^-23 each; the result is rounded to bfloat16, 2^-9).
+__device__ __forceinline__ float qt_silu(float z) {
+    float e, d;
+    asm("ex2.approx.f32 %0, %1;\n" : "=f"(e) : "f"(z * -1.4426950408889634f));
+    asm("rcp.approx.f32 %0, %1;\n" : "=f"(d) : "f"(1.f + e));
+    return z * d;
+}
 // Four products of 16 k: A in tensor memory (8 columns each), B in a swizzled K-major tile.
-__device__ __forceinline__ void qt_mma_step(unsigned d, unsigned a, unsigned b_lo, unsigned idesc, unsigned add) {
+__device__ __forceinline__ void qt_mma_64(unsigned d, unsigned a, unsigned b_lo, unsigned idesc, unsigned add) {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
         asm volatile("{\n .reg .pred p;\n .reg .b64 b;\n setp.ne.b32 p, %4, 0;\n mov.b64 b, {%2, %5};\n"
@@ -93,33 +104,40 @@ template <bool GATED, typename TO>
 __global__ void __launch_bounds__(QT_THREADS, 1)
 gemm_q4_tc_kernel(const __grid_constant__ QtMaps maps, const float* __restrict__ bias, TO* __restrict__ C, int M, int N, int blocks, int ldc, int act,
                   int group, int w_ready, const QtShape sh, int* __restrict__ error) {
-    constexpr int MATS = GATED ? 2 : 1;
+    constexpr int MATS = GATED ? 2 : 1, PLACES = GATED ? 2 : 4;   // (places: steps whose values there is room for)
     extern __shared__ unsigned char qt_raw[];
-    __shared__ __align__(8) unsigned long long full_bar[QT_MAX_STAGES], empty_bar[QT_MAX_STAGES], w_full[QT_PLACES], w_empty[QT_PLACES], acc_full, acc_empty;
+    __shared__ __align__(8) unsigned long long full_bar[QT_MAX_STAGES], empty_bar[QT_MAX_STAGES], w_full[PLACES], w_empty[PLACES], acc_full, acc_empty;
     __shared__ unsigned tmem_s;
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int split = sh.splits > 1 ? (int)tp_cluster_rank() : 0;
-    const unsigned x_bytes = (unsigned)sh.n * (TC_BK * 2), w_bytes = QT_CODES + (group == 32 ? 1024u : 512u);   // (loaded, a matrix)
-    const unsigned stage_bytes = x_bytes + MATS * (QT_CODES + QT_AFFINE);
+    const int group_shift = group == 32 ? 5 : (group == 64 ? 6 : 7);
+    const unsigned affine_row = (QT_K >> group_shift) * 64u;      // bytes of 16 rows' scales and offsets of a step
+    const unsigned x_room = (unsigned)sh.n * (QT_K * 2), stage_bytes = x_room + MATS * (QT_CODES + QT_AFFINE);
     const unsigned tiles = (tc_smem_u32(qt_raw) + 1023) & ~1023u;
-    const int kb0 = split * sh.kbs, nkb = min(blocks - kb0, sh.kbs);
-    const int xt = (M + sh.n - 1) / sh.n, total = (N + 127) / 128 * xt;
+    const int step0 = split * sh.steps, steps = min((blocks + 1) / 2 - step0, sh.steps);   // of this block's run
+    const int xt1 = (M + sh.n - 1) / sh.n, xt2 = (M + sh.n2 - 1) / sh.n2, main_tiles = sh.full_w * xt1;
+    const int total = main_tiles + ((N + 127) / 128 - sh.full_w) * xt2;
     const int me = (int)blockIdx.x / sh.splits, teams = (int)gridDim.x / sh.splits;
     const int my_tiles = (total - me + teams - 1) / teams;
-    // tiles that are worked on at the same time share rows of W
-    auto w0_of = [&](int ti) { return (me + ti * teams) / xt * 128; };
-    auto m0_of = [&](int ti) { return (me + ti * teams) % xt * sh.n; };
+    // (once a tile: divisions.  Once a load they were most of the producer's time.)  Tiles that are worked on at the same time share rows of W.
+    struct Tile { int w0, m0, n; };
+    auto tile_of = [&](int ti) {
+        const int i = me + ti * teams;
+        if (i < main_tiles) return Tile{i / xt1 * 128, i % xt1 * sh.n, sh.n};
+        return Tile{(sh.full_w + (i - main_tiles) / xt2) * 128, (i - main_tiles) % xt2 * sh.n2, sh.n2};
+    };
     if (threadIdx.x == 0) {
         for (int s = 0; s < sh.stages; ++s) {
             tc_mbar_init(tc_smem_u32(&full_bar[s]), 1);    // the producer, with the bytes
-            tc_mbar_init(tc_smem_u32(&empty_bar[s]), 1);   // the commit of the products that read the stage's x
+            // the commit of the products that read the stage's x; plain, the warps that make W's values too (see there)
+            tc_mbar_init(tc_smem_u32(&empty_bar[s]), GATED ? 1 : 1 + 4 * QT_TEAMS);
         }
-        for (int p = 0; p < QT_PLACES; ++p) {
-            tc_mbar_init(tc_smem_u32(&w_full[p]), 4);      // the four warps that fill it
-            tc_mbar_init(tc_smem_u32(&w_empty[p]), 1);     // the commit of the products that read it
+        for (int p = 0; p < PLACES; ++p) {
+            tc_mbar_init(tc_smem_u32(&w_full[p]), 8 * MATS);   // the warps that fill it
+            tc_mbar_init(tc_smem_u32(&w_empty[p]), 1);         // the commit of the products that read it
         }
         tc_mbar_init(tc_smem_u32(&acc_full), 1);
-        tc_mbar_init(tc_smem_u32(&acc_empty), 8);          // the epilogue's warps
+        tc_mbar_init(tc_smem_u32(&acc_empty), 8);              // the epilogue's warps
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     if (warp == 1) {
@@ -132,92 +150,115 @@ gemm_q4_tc_kernel(const __grid_constant__ QtMaps maps, const float* __restrict__
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
     const unsigned tmem = tmem_s;
 
-    auto load = [&](int ti, int kb, int s, bool of_w, bool of_x) {
+    auto load = [&](const Tile& tile, int step, int s, bool of_w, bool of_x) {
         const unsigned bar = tc_smem_u32(&full_bar[s]), st = tiles + (unsigned)s * stage_bytes;
+        const int k = (step0 + step) * QT_K;
         if (of_w) {
-            tc_mbar_expect_tx(bar, x_bytes + MATS * w_bytes);
+            tc_mbar_expect_tx(bar, (unsigned)tile.n * (QT_K * 2) + MATS * (QT_CODES + 8 * affine_row));
 #pragma unroll
             for (int i = 0; i < MATS; ++i) {
-                const unsigned at = st + x_bytes + i * (QT_CODES + QT_AFFINE);
-                tc_tma_load_2d(at, &maps.codes[i], (kb0 + kb) * Q4_BLOCK_WORDS, w0_of(ti) / 16, bar);
-                tc_tma_load_2d(at + QT_CODES, &maps.affine[i], (kb0 + kb) * 64 / group * 16, w0_of(ti) / 16, bar);
+                const unsigned at = st + x_room + i * (QT_CODES + QT_AFFINE);
+                tc_tma_load_2d(at, &maps.codes[i], k * 2, tile.w0 >> 4, bar);
+                tc_tma_load_2d(at + QT_CODES, &maps.affine[i], (k >> group_shift) * 16, tile.w0 >> 4, bar);
             }
         }
-        if (of_x) tc_tma_load_2d(st, &maps.x, (kb0 + kb) * TC_BK, m0_of(ti), bar);
+        if (of_x) {
+            const CUtensorMap* map = tile.n == sh.n ? &maps.x : &maps.x2;
+            tc_tma_load_2d(st, map, k, tile.m0, bar);
+            tc_tma_load_2d(st + (unsigned)tile.n * (TC_BK * 2), map, k + TC_BK, tile.m0, bar);
+        }
     };
-    const int ahead = w_ready ? min(sh.stages, nkb) : 0;   // stages whose W is asked for before the wait
+    const Tile tile0 = tile_of(0);
+    const int ahead = w_ready ? min(sh.stages, steps) : 0;   // stages whose W is asked for before the wait
     if (warp == 0)
-        for (int kb = 0; kb < ahead; ++kb)
-            if (tc_elect()) load(0, kb, kb, true, false);
+        for (int i = 0; i < ahead; ++i)
+            if (tc_elect()) load(tile0, i, i, true, false);
     pdl_wait();
     if (warp == 0)
-        for (int kb = 0; kb < ahead; ++kb)
-            if (tc_elect()) load(0, kb, kb, false, true);
+        for (int i = 0; i < ahead; ++i)
+            if (tc_elect()) load(tile0, i, i, false, true);
     __syncwarp();
     pdl_trigger();
 
     if (warp == 0) {
         int s = ahead == sh.stages ? 0 : ahead;
         unsigned phase = ahead == sh.stages ? 0 : 1;   // (the first time round a stage is free: the phase before the first has ended)
-        for (int ti = 0; ti < my_tiles; ++ti)
-            for (int kb = ti ? 0 : ahead; kb < nkb; ++kb) {
-                if (!tc_warp_wait(tc_smem_u32(&empty_bar[s]), phase)) {
+        for (int ti = 0; ti < my_tiles; ++ti) {
+            const Tile tile = tile_of(ti);
+            for (int i = ti ? 0 : ahead; i < steps; ++i) {
+                if (!qt_wait(tc_smem_u32(&empty_bar[s]), phase)) {
                     if (lane == 0) atomicExch(error, QT_ERR_PRODUCER);
                     ti = my_tiles;
                     break;
                 }
-                if (tc_elect()) load(ti, kb, s, true, true);
+                if (tc_elect()) load(tile, i, s, true, true);
                 if (++s == sh.stages) { s = 0; phase ^= 1; }
             }
+        }
     } else if (warp == 1) {
-        // float32 accumulator, bfloat16 operands, both K-major, N = n, M = 128
-        const unsigned idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(sh.n >> 3) << 17) | (8u << 24);
         int s = 0, place = 0;
         unsigned phase = 0, place_phase = 0;
         bool ok = true;
         for (int ti = 0; ok && ti < my_tiles; ++ti) {
-            ok = !ti || tc_warp_wait(tc_smem_u32(&acc_empty), (unsigned)((ti - 1) & 1));
-            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-            for (int kb = 0; ok && kb < nkb; ++kb) {
-                ok = tc_warp_wait(tc_smem_u32(&full_bar[s]), phase);
-                const unsigned xd = tc_desc_lo(tiles + (unsigned)s * stage_bytes);
+            const Tile tile = tile_of(ti);
+            // float32 accumulator, bfloat16 operands, both K-major, N = n, M = 128
+            const unsigned idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(tile.n >> 3) << 17) | (8u << 24);
+            const unsigned x_half = (unsigned)tile.n * (TC_BK * 2) >> 4;   // (in a descriptor's units)
+            ok = !ti || qt_wait(tc_smem_u32(&acc_empty), (unsigned)((ti - 1) & 1));
+            for (int i = 0; ok && i < steps; ++i) {
+                ok = qt_wait(tc_smem_u32(&full_bar[s]), phase) && qt_wait(tc_smem_u32(&w_full[place]), place_phase);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                const unsigned xd = tc_desc_lo(tiles + (unsigned)s * stage_bytes), a = tmem + QT_PLACES_AT + (unsigned)(place * MATS * 64);
+                if (tc_elect()) {
 #pragma unroll
-                for (int i = 0; i < MATS; ++i) {
-                    ok = ok && tc_warp_wait(tc_smem_u32(&w_full[place]), place_phase);
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-                    if (tc_elect()) {
-                        qt_mma_step(tmem + (unsigned)(i * sh.n), tmem + QT_PLACES_AT + place * 32, xd, idesc, kb > 0);
-                        tc_commit(tc_smem_u32(&w_empty[place]));
-                        if (i == MATS - 1) tc_commit(tc_smem_u32(&empty_bar[s]));
+                    for (int m = 0; m < MATS; ++m) {
+                        qt_mma_64(tmem + (unsigned)(m * sh.n), a + m * 64, xd, idesc, i > 0);
+                        qt_mma_64(tmem + (unsigned)(m * sh.n), a + m * 64 + 32, xd + x_half, idesc, 1u);
                     }
-                    if (++place == QT_PLACES) { place = 0; place_phase ^= 1; }
+                    tc_commit(tc_smem_u32(&w_empty[place]));
+                    tc_commit(tc_smem_u32(&empty_bar[s]));
                 }
+                if (++place == PLACES) { place = 0; place_phase ^= 1; }
                 if (++s == sh.stages) { s = 0; phase ^= 1; }
             }
             if (ok && tc_elect()) tc_commit(tc_smem_u32(&acc_full));
         }
         if (!ok && lane == 0) atomicExch(error, QT_ERR_MMA);
     } else if (warp < QT_EPILOGUE) {
+        constexpr int STRIDE = GATED ? 1 : 2;   // steps that a group goes on by
         const int team = (warp - QT_MAKERS) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
-        const unsigned codes_at = x_bytes + (GATED ? team * (QT_CODES + QT_AFFINE) : 0) + (row >> 4) * 512 + (row & 7) * 16 + (row >> 3 & 1) * 8;
-        const unsigned affine_at = x_bytes + (GATED ? team * (QT_CODES + QT_AFFINE) : 0) + QT_CODES + (row >> 4) * (group == 32 ? 128 : 64) +
-                                   (row & 7) * 8 + (row >> 3 & 1) * 4;
+        const int mat = GATED ? team & 1 : 0, part = GATED ? team >> 1 : team & 1;   // which half of a step
+        const unsigned w_at = tiles + x_room + mat * (QT_CODES + QT_AFFINE);
+        const unsigned codes_at = w_at + (row >> 4) * 1024 + part * 512 + (row & 7) * 16 + (row >> 3 & 1) * 8;
+        const unsigned affine_at = w_at + QT_CODES + (row >> 4) * affine_row + (part * 64 >> group_shift) * 64 + (row & 7) * 8 + (row >> 3 & 1) * 4;
         const unsigned second = group == 32 ? 64 : 0;   // (of 64 k the second half's group)
-        const unsigned lanes = tmem + QT_PLACES_AT + ((unsigned)(quarter * 32) << 16);
-        const int steps = my_tiles * nkb;
-        int s = GATED ? 0 : team % sh.stages, place = team;
+        const unsigned lanes = tmem + QT_PLACES_AT + mat * 64 + part * 32 + ((unsigned)(quarter * 32) << 16);
+        const int all = my_tiles * steps;
+        int i = GATED ? 0 : team >> 1, place = i, seen = 0, s = 0;
         unsigned phase = 0, place_phase = 1;   // (the first time round a place is free)
-        for (int i = GATED ? 0 : team; i < steps; i += GATED ? 1 : 2) {
-            if (!tc_warp_wait(tc_smem_u32(&full_bar[s]), phase)) {
-                if (lane == 0) atomicExch(error, QT_ERR_VALUES);
-                break;
+        uint2 q[4];
+        unsigned a0, a1, st = 0;
+        // Step `want`'s codes, scales and offsets from its stage.  Every step's mbarrier is waited for, in order, that of the other groups'
+        // steps too, and a stage is loaded again only when all have done so: who sees some of an mbarrier's phases only could take one for
+        // another, or miss one.  (Gated, every group has a part in every step, and no step's products begin without it.)
+        // `wait` false: only if it is there already.
+        auto fetch = [&](int want, bool wait) {
+            for (; seen <= want; ++seen) {
+                const unsigned bar = tc_smem_u32(&full_bar[s]);
+                if (!(wait ? qt_wait(bar, phase) : tc_warp_look(bar, phase))) return false;
+                if (!GATED && lane == 0) qt_arrive(tc_smem_u32(&empty_bar[s]));
+                st = (unsigned)s * stage_bytes;
+                if (++s == sh.stages) { s = 0; phase ^= 1; }
             }
-            const unsigned st = tiles + (unsigned)s * stage_bytes;
-            const unsigned a0 = qt_lds4(st + affine_at), a1 = qt_lds4(st + affine_at + second);
-            uint2 q[4];
+            a0 = qt_lds4(affine_at + st);
+            a1 = qt_lds4(affine_at + st + second);
 #pragma unroll
-            for (int t = 0; t < 4; ++t) q[t] = qt_lds8(st + codes_at + t * 128);
+            for (int t = 0; t < 4; ++t) q[t] = qt_lds8(codes_at + st + t * 128);
+            return true;
+        };
+        bool ok = i >= all || fetch(i, true);
+        for (; ok && i < all; i += STRIDE) {
             unsigned w[32];
             const unsigned s0 = q4_scale(a0), b0 = q4_offset(a0), s1 = q4_scale(a1), b1 = q4_offset(a1);
 #pragma unroll
@@ -228,20 +269,22 @@ gemm_q4_tc_kernel(const __grid_constant__ QtMaps maps, const float* __restrict__
                 q4_values(q[t].y, t < 2 ? s0 : s1, t < 2 ? b0 : b1, v);
                 w[8 * t + 4] = v[0]; w[8 * t + 5] = v[1]; w[8 * t + 6] = v[2]; w[8 * t + 7] = v[3];
             }
-            if (!tc_warp_wait(tc_smem_u32(&w_empty[place]), place_phase)) {
-                if (lane == 0) atomicExch(error, QT_ERR_VALUES);
-                break;
-            }
+            ok = qt_wait(tc_smem_u32(&w_empty[place]), place_phase);
+            if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-            qt_st32(lanes + place * 32, w);
+            qt_st32(lanes + place * (MATS * 64), w);
+            // The next step's codes while the values are on their way, if they have come.  (Waited for only behind the arrival: the ring may
+            // have no stage for them until this step's products have ended.)
+            const bool last = i + STRIDE >= all, there = !last && fetch(i + STRIDE, false);
+            asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
             __syncwarp();
             if (lane == 0) qt_arrive(tc_smem_u32(&w_full[place]));
-            place += 2;
-            if (place >= QT_PLACES) { place -= QT_PLACES; place_phase ^= 1; }
-            s += GATED ? 1 : 2;
-            if (s >= sh.stages) { s -= sh.stages; phase ^= 1; }
+            if (!last && !there) ok = fetch(i + STRIDE, true);
+            place += STRIDE;
+            if (place >= PLACES) { place -= PLACES; place_phase ^= 1; }
         }
+        if (!ok && lane == 0) atomicExch(error, QT_ERR_VALUES);
     } else {
         const int quarter = warp & 3, half = (warp - QT_EPILOGUE) >> 2;
         const int l = quarter * 32 + lane;   // this thread's row of the block's 128 rows of W
@@ -249,12 +292,13 @@ gemm_q4_tc_kernel(const __grid_constant__ QtMaps maps, const float* __restrict__
         bool ok = true;
         for (int ti = 0; ti < my_tiles; ++ti) {
             if (ok) {
-                ok = tc_warp_wait(tc_smem_u32(&acc_full), (unsigned)(ti & 1));
+                ok = qt_wait(tc_smem_u32(&acc_full), (unsigned)(ti & 1));
                 if (!ok && lane == 0) atomicExch(error, QT_ERR_EPILOGUE);
             }
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
             const unsigned acc = tmem + ((unsigned)(quarter * 32) << 16);
-            const int w0 = w0_of(ti), m0 = m0_of(ti), width = min(sh.n, M - m0), row = w0 + l;
+            const Tile tile = tile_of(ti);
+            const int m0 = tile.m0, width = min(tile.n, M - m0), row = tile.w0 + l;
             const float add = bias && row < N && sh.splits == 1 ? bias[row] : 0.f;
 #pragma unroll 1
             for (int c0 = half * 16; c0 < width; c0 += 32) {
@@ -278,10 +322,15 @@ gemm_q4_tc_kernel(const __grid_constant__ QtMaps maps, const float* __restrict__
                     continue;
                 }
                 float v[16];
+                if (!GATED) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const float a = __uint_as_float(r[0][j]);
-                    v[j] = GATED ? activation(a, act) * __uint_as_float(r[MATS - 1][j]) : a + add;
+                    for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[0][j]) + add;
+                } else if (act == VX_ACT_SILU) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[j] = qt_silu(__uint_as_float(r[0][j])) * __uint_as_float(r[MATS - 1][j]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[j] = activation(__uint_as_float(r[0][j]), act) * __uint_as_float(r[MATS - 1][j]);
                 }
                 TO* to = C + (size_t)(m0 + c0) * ldc;
                 if (sizeof(TO) == 2 && pairs) {
@@ -317,7 +366,7 @@ gemm_q4_tc_kernel(const __grid_constant__ QtMaps maps, const float* __restrict__
     }
     if (sh.splits > 1) {
         // each block adds its share of the columns, run after run
-        const int w0 = w0_of(0), m0 = m0_of(0);
+        const int w0 = tile0.w0, m0 = tile0.m0;
         const int width = min(sh.n, M - m0), c_end = min(width, (split + 1) * sh.n / sh.splits), c_beg = min(width, split * sh.n / sh.splits);
         for (int e = (int)threadIdx.x; e < (c_end - c_beg) * 128; e += QT_THREADS) {
             const int c = c_beg + (e >> 7), l = e & 127;
@@ -376,44 +425,47 @@ static int qt_launch(const QtMaps& maps, const float* bias, TO* C, int M, int N,
     return VX_OK;
 }
 
-// With a tile's shape: n a multiple of 16 up to 256 (gated 128), splits up to 8.  The other arguments as in vx_gemm_q4, checked there.
+// With a tile's shape: n a multiple of 16 up to 256 (gated 128), splits up to 8; without splits, the W tiles from full_w on may take tiles of n2 < n
+// rows of x (n2 0: none do).  The other arguments as in vx_gemm_q4.
 extern "C" int vx_gemm_q4_tc_shape(const void* x, const void* codes, const void* affine, const void* codes1, const void* affine1, const float* bias,
                                    void* out, int M, int N, int K, int ldx, int ldo, int group, int act, int out_dtype, int w_ready, int n,
-                                   int splits, int* error, cudaStream_t stream) {
+                                   int splits, int full_w, int n2, int* error, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return VX_OK;
-    const int mats = codes1 ? 2 : 1, blocks = (K + 63) / 64;
-    if (K <= 0 || !error || n < 16 || n > 256 / mats || (n & 15) || splits < 1 || splits > 8 || splits > blocks) return VX_ERR_SHAPE;
+    const int mats = codes1 ? 2 : 1, blocks = (K + 63) / 64, steps = (blocks + 1) / 2, wtiles = (N + 127) / 128;
+    if (K <= 0 || !error || n < 16 || n > 256 / mats || (n & 15) || splits < 1 || splits > 8 || splits > steps) return VX_ERR_SHAPE;
+    if (n2 && (splits > 1 || n2 < 16 || n2 > n || (n2 & 15) || full_w < 0 || full_w > wtiles)) return VX_ERR_SHAPE;
     if ((group != 32 && group != 64 && group != 128) || K % group || ldx < K || ldo < N) return VX_ERR_SHAPE;
     if (codes1 && (!affine1 || bias || act < 0 || act > VX_ACT_LAST)) return VX_ERR_SHAPE;
     if (out_dtype != VX_BF16 && (out_dtype != VX_F32 || codes1)) return VX_ERR_DTYPE;
     if (ldx & 7 || (((uintptr_t)x) | ((uintptr_t)codes) | ((uintptr_t)affine) | ((uintptr_t)codes1) | ((uintptr_t)affine1)) & 15) return VX_ERR_ALIGN;
     QtShape sh;
     sh.n = n;
-    sh.kbs = (blocks + splits - 1) / splits;
-    sh.splits = (blocks + sh.kbs - 1) / sh.kbs;   // (no run is empty)
-    const int stage = n * (TC_BK * 2) + mats * (QT_CODES + QT_AFFINE), stages = 220 * 1024 / stage;
+    sh.steps = (steps + splits - 1) / splits;
+    sh.splits = (steps + sh.steps - 1) / sh.steps;   // (no run is empty)
+    sh.full_w = n2 ? full_w : wtiles;
+    sh.n2 = n2 ? n2 : n;
+    const int stage = n * (QT_K * 2) + mats * (QT_CODES + QT_AFFINE), stages = QT_ROOM / stage;
     sh.stages = stages > QT_MAX_STAGES ? QT_MAX_STAGES : stages;
-    // An even number: plain, a group of makers then meets the same stages again and again, and sees every phase of their mbarriers.  (With
-    // an odd one it would wait for a stage's phase whose predecessor only the other group has seen end.)
-    sh.stages &= ~1;
     size_t bytes = (size_t)sh.stages * stage;
     const size_t sums = (size_t)mats * n * 512;
     if (sh.splits > 1 && bytes < sums) bytes = sums;
     if (bytes < 120 * 1024) bytes = 120 * 1024;   // (one block an SM: the tensor memory is one block's)
-    if (bytes > 222 * 1024) return VX_ERR_SHAPE;
     QtMaps maps;
     const long long wt = (N + 15) / 16, words = (long long)blocks * Q4_BLOCK_WORDS, pairs = (long long)blocks * 64 / group * 16;
-    const int box = group == 32 ? 32 : 16;
+    const int box = QT_K / group * 16;
     if (words > 0xffffffffLL) return VX_ERR_LIMIT;
-    if (!tc_make_map(&maps.x, x, M, K, ldx, n) || !qt_make_map(&maps.codes[0], codes, wt, words, Q4_BLOCK_WORDS) ||
+    if (!tc_make_map(&maps.x, x, M, K, ldx, n) || !qt_make_map(&maps.codes[0], codes, wt, words, 2 * Q4_BLOCK_WORDS) ||
         !qt_make_map(&maps.affine[0], affine, wt, pairs, box))
         return VX_ERR_DRIVER;
+    maps.x2 = maps.x;
+    if (sh.n2 != n && !tc_make_map(&maps.x2, x, M, K, ldx, sh.n2)) return VX_ERR_DRIVER;
     maps.codes[1] = maps.codes[0];
     maps.affine[1] = maps.affine[0];
-    if (codes1 && (!qt_make_map(&maps.codes[1], codes1, wt, words, Q4_BLOCK_WORDS) || !qt_make_map(&maps.affine[1], affine1, wt, pairs, box))) return VX_ERR_DRIVER;
+    if (codes1 && (!qt_make_map(&maps.codes[1], codes1, wt, words, 2 * Q4_BLOCK_WORDS) || !qt_make_map(&maps.affine[1], affine1, wt, pairs, box)))
+        return VX_ERR_DRIVER;
     static int sm_counts[VX_MAX_DEVICES];
     const int sms = vx_sm_count(sm_counts);
-    const long long tiles = (long long)((N + 127) / 128) * ((M + n - 1) / n);
+    const long long tiles = (long long)sh.full_w * ((M + n - 1) / n) + (long long)(wtiles - sh.full_w) * ((M + sh.n2 - 1) / sh.n2);
     if (tiles > 0x7fffff) return VX_ERR_LIMIT;
     const int teams = sh.splits > 1 ? (int)tiles : (int)(tiles < sms ? tiles : sms);
 #define QT_GO(G_, T_) qt_launch<G_, T_>(maps, bias, (T_*)out, M, N, blocks, ldo, act, group, w_ready, sh, bytes + 1024, teams, error, stream)
@@ -431,7 +483,7 @@ extern "C" int vx_gemm_q4_tc(const void* x, const void* codes, const void* affin
     const int sms = vx_sm_count(sm_counts), most = codes1 ? 128 : 256, blocks = (K + 63) / 64;
     const int xt = (M + most - 1) / most, n = ((M + xt - 1) / xt + 15) & ~15, tiles = (N + 127) / 128 * xt;
     int splits = sms / tiles;
-    if (splits > blocks / 4) splits = blocks / 4;
+    if (splits > blocks / 8) splits = blocks / 8;
     splits = splits < 1 ? 1 : (splits > 8 ? 8 : splits);
-    return vx_gemm_q4_tc_shape(x, codes, affine, codes1, affine1, bias, out, M, N, K, ldx, ldo, group, act, out_dtype, w_ready, n, splits, error, stream);
+    return vx_gemm_q4_tc_shape(x, codes, affine, codes1, affine1, bias, out, M, N, K, ldx, ldo, group, act, out_dtype, w_ready, n, splits, 0, 0, error, stream);
 }

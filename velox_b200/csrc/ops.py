@@ -197,7 +197,7 @@ def _declare(lib) -> None:
         "vx_quantize_q4": [P, P, P, I, I, c_longlong, I, I, P],
         "vx_dequantize_q4": [P, P, P, I, I, I, P],
         "vx_gemm_q4": [P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, P, P],
-        "vx_gemm_q4_tc_shape": [P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, P, P],
+        "vx_gemm_q4_tc_shape": [P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, I, I, P, P],
     }
     lib.vx_set_pdl_mask.argtypes = [I]
     lib.vx_host_word.argtypes, lib.vx_host_word.restype = [], c_void_p
@@ -1968,7 +1968,7 @@ def gemm_bf16(a: torch.Tensor, w: torch.Tensor, bias=None, out_dtype: Optional[t
 
 
 Q4_GROUPS = (32, 64, 128)   # neighbours along a row that share a scale and an offset
-Q4_FEW_ROWS = 8             # rows up to which the products stream the matrix through mma.sync; above they have bounded waits
+Q4_FEW_ROWS = 16            # rows up to which the products stream the matrix through mma.sync; above they have bounded waits
 
 
 class Q4Matrix:
@@ -1987,6 +1987,13 @@ class Q4Matrix:
         _need(codes.device == affine.device, "Q4Matrix: codes on %s, scales and offsets on %s" % (codes.device, affine.device))
         _need(codes.data_ptr() % 16 == 0 and affine.data_ptr() % 16 == 0, "Q4Matrix: 16-byte aligned tensors")
         self.codes, self.affine, self.rows, self.depth, self.group = codes, affine, int(rows), int(depth), int(group)
+
+    @classmethod
+    def _of(cls, codes, affine, rows, depth, group):
+        """(Tensors that a kernel has just laid out.)"""
+        m = cls.__new__(cls)
+        m.codes, m.affine, m.rows, m.depth, m.group = codes, affine, rows, depth, group
+        return m
 
     @property
     def shape(self) -> Tuple[int, int]:
@@ -2019,6 +2026,11 @@ def quantize_q4(w: torch.Tensor, group: int = 64) -> Q4Matrix:
     """`w` [N, K] (bfloat16 or float32, rows 16-byte aligned, K a multiple of `group`) in four bits: per group of neighbours
     s = bfloat16((max - min) / 15), b = bfloat16(min), q = round((w - b) / s) within 0 to 15 (ties to even; s = 0: q = 0).  A group with a value
     that is not finite, or whose scale is not, stands for NaN."""
+    if w.is_cuda:
+        out = (_CALLS or _calls()).quantize_q4(w, group)
+        if out is not None:
+            codes, affine = _called(out, "quantize_q4")
+            return Q4Matrix._of(codes, affine, w.shape[0], w.shape[1], group)
     _dev(w)
     _need(w.dim() == 2 and w.dtype in (torch.bfloat16, torch.float32) and w.stride(1) == 1, "quantize_q4: bfloat16 or float32 w [N, K], rows contiguous")
     n, k = w.shape
@@ -2030,11 +2042,15 @@ def quantize_q4(w: torch.Tensor, group: int = 64) -> Q4Matrix:
     affine = torch.empty((tiles, groups, 8, 2, 2), dtype=torch.bfloat16, device=w.device)
     _check(library().vx_quantize_q4(_ptr(w), _ptr(codes), _ptr(affine), n, k, w.stride(0) if n > 1 else k, group, dtype_code(w.dtype), _stream()),
            "quantize_q4")
-    return Q4Matrix(codes, affine, n, k, group)
+    return Q4Matrix._of(codes, affine, n, k, group)
 
 
 def dequantize_q4(w: Q4Matrix) -> torch.Tensor:
     """The bfloat16 matrix that `w` stands for: what the products multiply with."""
+    if w.codes.is_cuda:
+        out = (_CALLS or _calls()).dequantize_q4(w.codes, w.affine, w.rows, w.depth, w.group)
+        if out is not None:
+            return _called(out, "dequantize_q4")
     _dev(w.codes, w.affine)
     if _elsewhere(w.codes):
         with torch.cuda.device(w.device):
@@ -2045,6 +2061,14 @@ def dequantize_q4(w: Q4Matrix) -> torch.Tensor:
 
 
 def _q4_product(what: str, a: torch.Tensor, w: Q4Matrix, up: Optional[Q4Matrix], bias, out_dtype, act: int, w_ready: bool) -> torch.Tensor:
+    if a.is_cuda:
+        out = (_CALLS or _calls()).gemm_q4(a, w.codes, w.affine, up.codes if up is not None else None, up.affine if up is not None else None,
+                                           bias, w.rows, w.depth, w.group, act, out_dtype, 1 if w_ready else 0, _error_address(a.device))
+        if out is not None:
+            out = _called(out, what)
+            if out.shape[0] > Q4_FEW_ROWS:
+                note_bounded_wait()
+            return out
     _dev(a, w.codes, w.affine, bias)
     _need(a.dtype == torch.bfloat16 and a.dim() == 2 and a.shape[1] == w.depth, "%s: bfloat16 a [M, %d]" % (what, w.depth))
     m, k = a.shape

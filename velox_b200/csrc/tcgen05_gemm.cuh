@@ -37,10 +37,18 @@ __device__ __forceinline__ bool tc_mbar_wait(unsigned bar, unsigned parity) {
 // A bounded wait of a whole warp, with one answer for all its lanes.  A role that goes on as a warp (tc_elect, tcgen05.ld) waits this
 // way: if lanes counted by themselves, a phase that ends as the limit does could let some of them through and send others away, and an
 // elect.sync that names lanes which have left is undefined.
-__device__ __forceinline__ bool tc_warp_wait(unsigned bar, unsigned parity) {
-    for (int i = 0; i < TC_SPIN_LIMIT; ++i)
+__device__ __forceinline__ bool tc_warp_wait(unsigned bar, unsigned parity, int limit = TC_SPIN_LIMIT) {
+    for (int i = 0; i < limit; ++i)
         if (__all_sync(0xffffffffu, tc_mbar_try(bar, parity))) return true;
     return false;
+}
+// One look, with one answer for the warp.  (`try_wait` sleeps for a while where the phase has not ended, `test_wait` does not.)
+__device__ __forceinline__ bool tc_warp_look(unsigned bar, unsigned parity) {
+    unsigned ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return __all_sync(0xffffffffu, ok != 0);
 }
 __device__ __forceinline__ void tc_tma_load_2d(unsigned dst, const CUtensorMap* map, int x, int y, unsigned bar) {
     asm volatile(
