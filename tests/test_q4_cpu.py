@@ -57,3 +57,48 @@ def test_the_entry_points_refuse_before_they_launch():
         assert made(**change) == code, change
     assert lib.vx_dequantize_q4(A, A, A, 0, 128, 64, None) == 0
     assert lib.vx_dequantize_q4(A, A, A, 32, 96, 64, None) == SHAPE and lib.vx_dequantize_q4(A, A, A + 2, 32, 128, 64, None) == ALIGN
+
+
+def test_engine_settings():
+    from velox_b200 import EngineConfig
+    cfg = EngineConfig(weight_bits=4, weight_group=128, head_bits=4)
+    assert (cfg.weight_bits, cfg.weight_group, cfg.head_bits) == (4, 128, 4)
+    assert EngineConfig().weight_bits is None and EngineConfig().head_bits is None
+    for kw, why in [(dict(weight_bits=8), "weight_bits"), (dict(weight_bits=0), "weight_bits"), (dict(head_bits=2), "head_bits"),
+                    (dict(weight_bits=4, weight_group=48), "weight_group"), (dict(weight_bits=4, dtype="float32"), "bfloat16"),
+                    (dict(head_bits=4, dtype="float32"), "bfloat16")]:
+        with pytest.raises(ValueError, match=why):
+            EngineConfig(**kw)
+
+
+def test_which_parts_can_hold_four_bits():
+    from helpers import tiny_config
+    from velox_b200.config.registry import resolve_architecture
+    from velox_b200.models.decoder import DecoderModel
+    cfg = tiny_config("tiny_b")
+    assert DecoderModel(resolve_architecture(cfg.to_dict()).plan(cfg)).without_four_bits() == []
+    from dobepel_helpers import CONFIGS
+    raw = CONFIGS["even"]
+    arch = resolve_architecture(raw)
+    others = DecoderModel(arch.plan(arch.config_class.from_dict(raw))).without_four_bits()
+    assert others and "PagedAttention" not in others and "GatedMLP" not in others
+
+
+def test_rows_that_do_not_go_into_groups_are_named():
+    from velox_b200.parts.linear import Linear, linear
+    w = torch.zeros(16, 160)
+    assert isinstance(linear(w), Linear)
+    with pytest.raises(ValueError, match=r"down_proj: rows of 160 do not go into four-bit groups of 64; they go into groups of \[32\]"):
+        linear(w, None, 64, "down_proj")
+    with pytest.raises(ValueError, match="none of the sizes"):
+        linear(torch.zeros(16, 40), None, 32, "w")
+
+
+def test_the_command_line_names_the_settings():
+    from velox_b200.cli import build_parser
+    args = build_parser().parse_args(["generate", "--weight-bits", "4", "--weight-group", "128", "--head-bits", "4"])
+    assert (args.weight_bits, args.weight_group, args.head_bits) == (4, 128, 4)
+    args = build_parser().parse_args(["generate"])
+    assert args.weight_bits is None and args.head_bits is None and args.weight_group == 64
+    with pytest.raises(SystemExit):
+        build_parser().parse_args(["generate", "--weight-bits", "8"])

@@ -88,7 +88,8 @@ def cmd_generate(args) -> int:
         raise SystemExit("give --prompt-tokens 1,2,3 (repeatable) or --prompt-lens 5,11,17")
     cfg = EngineConfig(dtype=args.dtype, device=args.device, page_size=args.page_size, num_pages=args.num_pages,
                        max_running_requests=args.max_concurrent, max_batch_tokens=args.max_batch_tokens,
-                       chunk_size=args.chunk_size, max_model_len=args.max_model_len, seed=args.seed)
+                       chunk_size=args.chunk_size, max_model_len=args.max_model_len, seed=args.seed,
+                       weight_bits=args.weight_bits, weight_group=args.weight_group, head_bits=args.head_bits)
     limit = _memory_bytes(args.max_model_memory, torch.device(args.device))
     engine = Engine(folder, cfg, cache_memory_limit=limit)
     stops = [[int(t) for t in q.split(",") if t.strip()] for q in (args.stop or [])]
@@ -143,6 +144,10 @@ def build_parser() -> argparse.ArgumentParser:
     g.add_argument("--stop", action="append", help="comma-separated token ids; generation stops after this run of "
                                                     "tokens (may be given several times)")
     g.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
+    g.add_argument("--weight-bits", type=int, choices=[4], default=None,
+                   help="hold the layers' matrices in four bits, made as they are loaded (default: as the --dtype)")
+    g.add_argument("--weight-group", type=int, choices=[32, 64, 128], default=64, help="neighbours of a row that share a scale and an offset")
+    g.add_argument("--head-bits", type=int, choices=[4], default=None, help="the same for the output head")
     g.add_argument("--device", default="cuda:0")
     g.add_argument("--page-size", type=int, default=16)
     g.add_argument("--num-pages", type=int, default=None)

@@ -68,7 +68,8 @@ class Engine:
             raise RuntimeError("velox_b200 runs on a CUDA device (sm_100a); none is visible")
         self.device = torch.device(self.config.device)
         torch.cuda.set_device(self.device)
-        self.runtime = Runtime(_TORCH_DTYPES[self.config.dtype], self.device)
+        self.runtime = Runtime(_TORCH_DTYPES[self.config.dtype], self.device, self.config.weight_group if self.config.weight_bits else 0,
+                               self.config.weight_group if self.config.head_bits else 0)
         if model_dir is not None:
             self.architecture, self.model_config = load_config(model_dir)
             with open(os.path.join(model_dir, "config.json")) as f:
@@ -81,6 +82,11 @@ class Engine:
             self.architecture = resolve_architecture(raw)
         self.plan = self.architecture.plan(self.model_config)
         self.model = DecoderModel(self.plan)
+        if self.runtime.weight_group and self.model.without_four_bits():
+            raise ValueError("weight_bits=4: %s hold their matrices in the engine's element type only"
+                             % ", ".join(self.model.without_four_bits()))
+        if self.runtime.head_group and not self.model.head.four_bit_weights:
+            raise ValueError("head_bits=4: %s holds its matrix in the engine's element type only" % type(self.model.head).__name__)
         if model_dir is not None:
             load_weights(self.model, model_dir, self.runtime)
         else:

@@ -69,6 +69,10 @@ class DecoderModel:
         self.probe = None
         self.runtime: Optional[Runtime] = None
 
+    def without_four_bits(self) -> List[str]:
+        """The kinds of mixers and feed-forwards whose matrices can't be held in four bits."""
+        return sorted({type(p).__name__ for b in self.blocks for p in (b.mixer, b.feed_forward) if p is not None and not p.four_bit_weights})
+
     # -- weights -------------------------------------------------------------
     def parts(self) -> List[Part]:
         out: List[Part] = [self.embedding]

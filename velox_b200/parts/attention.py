@@ -55,7 +55,7 @@ import torch
 
 from ..csrc import ops
 from .base import Mixer, PagedKV, Runtime, TensorSpec
-from .linear import Linear
+from .linear import Linear, linear
 from .plan import PartSpec
 from .registry import build_part
 
@@ -70,6 +70,7 @@ class PagedAttention(Mixer):
     # such a portion one block per kv head that walks ALL the request's keys alone: 16 tokens on top of
     # 4,000 cached keys took 300 us a layer that way.
     short_rows_up_to = TC_PREFILL_MIN_TOKENS - 1
+    four_bit_weights = True
 
     @property
     def cuda_graph_safe(self) -> bool:
@@ -193,12 +194,12 @@ class PagedAttention(Mixer):
         w = torch.cat(mats, dim=0).contiguous()
         b = torch.cat(biases).contiguous() if biases is not None else None
         del mats
-        self.qkv = Linear(w, b)
+        self.qkv = linear(w, b, runtime.weight_group, "%sprojections" % self.prefix)
         if self.sink:
             self.sinks = tensors[self.sink_name].to(torch.float32).contiguous()
         elif self.sink_value is not None:
             self.sinks = torch.full((self.num_heads,), self.sink_value, dtype=torch.float32, device=runtime.device)
-        self.out = Linear(tensors[self._w("o_proj")], tensors[self._b("o_proj")] if self.out_bias else None)
+        self.out = linear(tensors[self._w("o_proj")], tensors[self._b("o_proj")] if self.out_bias else None, runtime.weight_group, self._w("o_proj"))
         if self.qk_norm and not self.qk_norm_weight:   # (the kernels read a multiplier per channel)
             self.q_norm_weight = torch.ones(self.head_dim, dtype=torch.float32, device=runtime.device)
             self.k_norm_weight = self.q_norm_weight if self.own_kv else None

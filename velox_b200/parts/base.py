@@ -51,8 +51,12 @@ class TensorSpec:
 
 @dataclass(frozen=True)
 class Runtime:
+    """What parts are bound for.  `weight_group` > 0: a part that can (`four_bit_weights`) holds its matrices in four bits, in groups of so
+    many neighbours of a row; `head_group`: the same for an output head."""
     dtype: torch.dtype
     device: torch.device
+    weight_group: int = 0
+    head_group: int = 0
 
 
 @dataclass(frozen=True)
@@ -117,6 +121,8 @@ class Part:
     # are fixed for a given batch size): only then may a step be captured in a
     # CUDA graph.  Parts that look at the step's host-side lists leave it False.
     cuda_graph_safe = False
+    # True if the part holds its matrices in four bits where `Runtime.weight_group` (a head: `head_group`) asks for it.
+    four_bit_weights = False
 
     def __init__(self, prefix: str = ""):
         self.prefix = prefix

@@ -16,7 +16,7 @@ import torch
 
 from ..csrc import ops
 from .base import Embedding, FixedState, Part, Runtime, TensorSpec
-from .linear import matmul
+from .linear import linear, matmul
 
 
 class TokenEmbedding(Embedding):
@@ -85,6 +85,7 @@ class PairHashEmbedding(Embedding):
 
 class OutputHead(Part):
     cuda_graph_safe = True  # reads nothing of a step but device tensors and sizes fixed per graph
+    four_bit_weights = True
 
     def __init__(self, prefix: str, vocab_size: int, hidden_size: int, tied: bool = False, weight_name: str = "weight",
                  logit_scale: float = 1.0, logit_softcap: float = 0.0):
@@ -94,6 +95,7 @@ class OutputHead(Part):
         self.logit_scale = float(logit_scale)
         self.weight_name = prefix + weight_name
         self.weight: Optional[torch.Tensor] = None
+        self.q4 = None
 
     def tensor_specs(self) -> List[TensorSpec]:
         if self.tied:
@@ -107,13 +109,17 @@ class OutputHead(Part):
     def bind(self, tensors: Dict[str, torch.Tensor], runtime: Runtime) -> None:
         super().bind(tensors, runtime)
         if not self.tied:
-            self.weight = tensors[self.weight_name]
+            self._take(tensors[self.weight_name])
 
     def tie(self, table: torch.Tensor) -> None:
-        self.weight = table
+        self._take(table)
+
+    def _take(self, weight: torch.Tensor) -> None:
+        self.q4 = linear(weight, None, self.runtime.head_group, self.weight_name) if self.runtime.head_group else None
+        self.weight = weight if self.q4 is None else None
 
     def forward(self, rows: torch.Tensor) -> torch.Tensor:
-        logits = matmul(rows, self.weight, None, torch.float32)
+        logits = matmul(rows, self.weight, None, torch.float32) if self.q4 is None else self.q4(rows, torch.float32)
         if self.logit_scale != 1.0:
             logits = ops.scale_rows(logits, self.logit_scale)
         return ops.softcap_rows(logits, self.logit_softcap) if self.logit_softcap > 0 else logits

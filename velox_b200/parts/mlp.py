@@ -5,7 +5,8 @@ followed by the 8 up rows of the same features, so that a matrix-product kernel
 that owns a tile holds gate and up of a feature together and can apply
 act(gate) * up before anything is written (if the intermediate size is no
 multiple of 8, all gate rows are followed by all up rows and the product is taken
-by a kernel of its own).  Activation and product are formed in float32.
+by a kernel of its own).  Activation and product are formed in float32.  Held in four
+bits gate and up stay two matrices, which one kernel reads side by side.
 """
 from __future__ import annotations
 
@@ -15,7 +16,7 @@ import torch
 
 from ..csrc import ops
 from .base import FeedForward, Runtime, TensorSpec
-from .linear import Linear
+from .linear import Linear, linear
 
 
 GATE_TILE = 8
@@ -24,6 +25,7 @@ FUSED_TCGEN05_MIN_ROWS = 128
 
 class GatedMLP(FeedForward):
     cuda_graph_safe = True  # reads nothing of a step but device tensors and sizes fixed per graph
+    four_bit_weights = True
 
     def __init__(self, prefix: str, hidden_size: int, intermediate_size: int, activation: str = "silu",
                  names: Sequence[str] = ("gate_proj.weight", "up_proj.weight", "down_proj.weight")):
@@ -46,6 +48,12 @@ class GatedMLP(FeedForward):
         p = self.prefix
         gate, up = tensors[self.names[0]], tensors[self.names[1]]
         i, e = self.intermediate_size, self.hidden_size
+        self.pair = None
+        if runtime.weight_group:   # (the kernels hold gate and up of a feature together whatever their order in memory)
+            self.pair = tuple(linear(w, None, runtime.weight_group, n).matrix for w, n in ((gate, self.names[0]), (up, self.names[1])))
+            del gate, up
+            self.down = linear(tensors[self.names[2]], None, runtime.weight_group, self.names[2])
+            return
         if i % GATE_TILE == 0:
             self.tile = GATE_TILE
             w = torch.stack([gate.view(i // GATE_TILE, GATE_TILE, e), up.view(i // GATE_TILE, GATE_TILE, e)], 1)
@@ -56,6 +64,8 @@ class GatedMLP(FeedForward):
         self.down = Linear(tensors[self.names[2]])
 
     def forward(self, h: torch.Tensor, ctx=None) -> torch.Tensor:
+        if self.pair is not None:
+            return self.down(ops.gated_q4(h, self.pair[0], self.pair[1], self.activation, w_ready=True))
         w = self.gate_up.weight
         fused = self.tile and h.dtype == torch.bfloat16
         rows = h.shape[0]
