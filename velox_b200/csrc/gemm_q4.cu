@@ -43,6 +43,11 @@ template <int FORM, int GROUP, int BLOCKS> struct Q4Step {
     static constexpr int mats = FORM == Q4_ONE ? 1 : 2, codes = BLOCKS * 512, affine = BLOCKS * 64 * 64 / GROUP, bytes = codes + affine;
 };
 
+// The warps' sums of a tile, in shared memory: two buffers where they are small.
+template <int FORM, int NT, int WARPS> struct Q4Sums {
+    static constexpr int buffers = NT > 2 ? 1 : 2, bytes = buffers * (FORM == Q4_ONE ? 1 : 2) * WARPS * 16 * (8 * NT + 1) * 4;
+};
+
 template <int FORM, typename TO, int GROUP, int NT, int WARPS, int BLOCKS, int DEPTH, int PER_SM>
 __global__ void __launch_bounds__(WARPS * 32, PER_SM)
 gemm_q4_kernel(const bf16* __restrict__ x, const Q4Pair w, const float* __restrict__ bias, TO* __restrict__ out, int M, int N, int K, int ldx,
@@ -52,7 +57,9 @@ gemm_q4_kernel(const bf16* __restrict__ x, const Q4Pair w, const float* __restri
     static_assert(BLOCKS * 64 % GROUP == 0, "a step holds whole groups");
     constexpr int MATS = Step::mats, SLOT = MATS * Step::bytes;
     extern __shared__ __align__(16) unsigned char q4_ring[];
-    __shared__ float red[2][MATS][WARPS][16][8 * NT + 1];
+    constexpr int RED = Q4Sums<FORM, NT, WARPS>::buffers;
+    typedef float Sums[MATS][WARPS][16][8 * NT + 1];
+    Sums* red = reinterpret_cast<Sums*>(q4_ring + WARPS * DEPTH * SLOT);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
     // the warp's code blocks of a tile: neighbours, as many for every warp as there can be (whole groups)
     constexpr int UNIT = GROUP == 128 ? 2 : 1;
@@ -177,7 +184,7 @@ gemm_q4_kernel(const bf16* __restrict__ x, const Q4Pair w, const float* __restri
 #pragma unroll
         for (int j = 0; j < NT; ++j) xr[j] -= (mine + BLOCKS - 1) / BLOCKS * (BLOCKS * 64);
         // a lane holds out^T[row r (0, 1) and r + 8 (2, 3)][rows 2 t, 2 t + 1 of x]
-        const int buf = ti & 1;
+        const int buf = ti & (RED - 1);
 #pragma unroll
         for (int i = 0; i < MATS; ++i)
 #pragma unroll
@@ -187,7 +194,7 @@ gemm_q4_kernel(const bf16* __restrict__ x, const Q4Pair w, const float* __restri
                     const int m = 8 * n + 2 * t + (j & 1);
                     if (m < M) red[buf][i][warp][r + 8 * (j >> 1)][m] = acc[i][n][j];
                 }
-        __syncthreads();   // (the sums that are read here are overwritten after the next of these)
+        __syncthreads();   // (with two buffers the sums that are read here are overwritten after the next of these)
         const int unit = blockIdx.x + ti * gridDim.x;
         constexpr int ROWS = TWO ? 32 : 16;
         for (int e = threadIdx.x; e < ROWS * M; e += WARPS * 32) {
@@ -203,6 +210,7 @@ gemm_q4_kernel(const bf16* __restrict__ x, const Q4Pair w, const float* __restri
                 out[(size_t)m * ldo + n] = from_f32<TO>(GATED ? activation(v, act) * up : v);
             }
         }
+        if (RED == 1) __syncthreads();
     }
     asm volatile("cp.async.wait_all;\n" ::: "memory");
 }
@@ -217,7 +225,7 @@ static int q4_go(const bf16* x, const Q4Pair& w, const float* bias, TO* out, int
                  cudaStream_t stream) {
     typedef Q4Step<FORM, GROUP, BLOCKS> Step;
     const int blocks = (K + 63) / 64, rows = FORM == Q4_TWO ? 32 : 16, units = (N + rows - 1) / rows, room = q4_sms() * PER_SM;
-    const size_t smem = (size_t)WARPS * DEPTH * Step::mats * Step::bytes;
+    const size_t smem = (size_t)WARPS * DEPTH * Step::mats * Step::bytes + Q4Sums<FORM, NT, WARPS>::bytes;
     auto kernel = gemm_q4_kernel<FORM, TO, GROUP, NT, WARPS, BLOCKS, DEPTH, PER_SM>;
     static bool configured[VX_MAX_DEVICES];
     if (int rc = vx_configure_smem(kernel, smem, configured)) return rc;
@@ -244,7 +252,10 @@ static int q4_launch(const bf16* x, const Q4Pair& w, const float* bias, TO* out,
 #undef Q4_GO
 }
 
-#define Q4_FEW_ROWS 16
+// Rows up to which the kernel above is taken: 16, or 32 where the matrix is small.  us, this way and on tcgen05: 16 rows 4096 x 4096 5.9, 9.6; gated
+// 12288 x 4096 22.8, 24.8; gated 17408 x 5120 33.5, 31.1; 32 rows 2048 x 2048 3.7, 5.9; 4096 x 4096 8.7, 9.6; 6144 x 4096 12.3, 11.8; 7168 x 5120
+// 15.3, 14.0; gated 9728 x 2560 23.0, 16.8; 24 rows 6144 x 4096 11.3, 11.8; 4096 x 12288 18.9, 15.8.
+static bool q4_few(int M, int N, int K, bool gated) { return M <= 16 || (M <= 32 && (long long)N * K * (gated ? 2 : 1) <= 26000000LL); }
 
 extern "C" int vx_gemm_q4_tc(const void* x, const void* codes, const void* affine, const void* codes1, const void* affine1, const float* bias,
                              void* out, int M, int N, int K, int ldx, int ldo, int group, int act, int out_dtype, int w_ready, int* error,
@@ -259,11 +270,11 @@ extern "C" int vx_gemm_q4(const void* x, const void* codes, const void* affine, 
     if (K <= 0 || (group != 32 && group != 64 && group != 128) || K % group || ldx < K || ldo < N) return VX_ERR_SHAPE;
     if (codes1 && (!affine1 || bias || act < 0 || act > VX_ACT_LAST)) return VX_ERR_SHAPE;
     if (ldx & 7 || (((uintptr_t)x) | ((uintptr_t)codes) | ((uintptr_t)affine) | ((uintptr_t)codes1) | ((uintptr_t)affine1)) & 15) return VX_ERR_ALIGN;
-    if (M > Q4_FEW_ROWS)
+    if (!q4_few(M, N, K, codes1 != nullptr))
         return vx_gemm_q4_tc(x, codes, affine, codes1, affine1, bias, out, M, N, K, ldx, ldo, group, act, out_dtype, w_ready, error, stream);
     const Q4Pair w = {{(const unsigned*)codes, (const unsigned*)codes1}, {(const unsigned*)affine, (const unsigned*)affine1}};
 #define Q4_ROWS(G, T, GR, NT) q4_launch<G, T, GR, NT>((const bf16*)x, w, bias, (T*)out, M, N, K, ldx, ldo, act, w_ready, stream)
-#define Q4_GROUP(G, T, GR) (M <= 8 ? Q4_ROWS(G, T, GR, 1) : Q4_ROWS(G, T, GR, 2))
+#define Q4_GROUP(G, T, GR) (M <= 8 ? Q4_ROWS(G, T, GR, 1) : (M <= 16 ? Q4_ROWS(G, T, GR, 2) : Q4_ROWS(G, T, GR, 4)))
 #define Q4_CALL(G, T) (group == 32 ? Q4_GROUP(G, T, 32) : (group == 64 ? Q4_GROUP(G, T, 64) : Q4_GROUP(G, T, 128)))
     if (out_dtype == VX_BF16) return codes1 ? Q4_CALL(true, bf16) : Q4_CALL(false, bf16);
     if (out_dtype == VX_F32) return codes1 ? VX_ERR_DTYPE : Q4_CALL(false, float);

@@ -42,10 +42,9 @@ struct QtShape {
     int n;             // rows of x in a tile
     int splits;        // runs of k
     int steps;         // steps of a run
-    int full_w, n2;    // W tiles from full_w on take tiles of n2 rows of x (full_w: all of them, where none do)
     int stages;
 };
-struct QtMaps { CUtensorMap x, x2, codes[2], affine[2]; };
+struct QtMaps { CUtensorMap x, codes[2], affine[2]; };
 
 __device__ __forceinline__ void qt_st32(unsigned taddr, const unsigned (&r)[32]) {
     asm volatile(
@@ -115,16 +114,14 @@ gemm_q4_tc_kernel(const __grid_constant__ QtMaps maps, const float* __restrict__
     const unsigned x_room = (unsigned)sh.n * (QT_K * 2), stage_bytes = x_room + MATS * (QT_CODES + QT_AFFINE);
     const unsigned tiles = (tc_smem_u32(qt_raw) + 1023) & ~1023u;
     const int step0 = split * sh.steps, steps = min((blocks + 1) / 2 - step0, sh.steps);   // of this block's run
-    const int xt1 = (M + sh.n - 1) / sh.n, xt2 = (M + sh.n2 - 1) / sh.n2, main_tiles = sh.full_w * xt1;
-    const int total = main_tiles + ((N + 127) / 128 - sh.full_w) * xt2;
+    const int xt = (M + sh.n - 1) / sh.n, total = (N + 127) / 128 * xt;
     const int me = (int)blockIdx.x / sh.splits, teams = (int)gridDim.x / sh.splits;
     const int my_tiles = (total - me + teams - 1) / teams;
     // (once a tile: divisions.  Once a load they were most of the producer's time.)  Tiles that are worked on at the same time share rows of W.
-    struct Tile { int w0, m0, n; };
+    struct Tile { int w0, m0; };
     auto tile_of = [&](int ti) {
-        const int i = me + ti * teams;
-        if (i < main_tiles) return Tile{i / xt1 * 128, i % xt1 * sh.n, sh.n};
-        return Tile{(sh.full_w + (i - main_tiles) / xt2) * 128, (i - main_tiles) % xt2 * sh.n2, sh.n2};
+        const int i = me + ti * teams, row = i / xt;
+        return Tile{row * 128, (i - row * xt) * sh.n};
     };
     if (threadIdx.x == 0) {
         for (int s = 0; s < sh.stages; ++s) {
@@ -154,7 +151,7 @@ gemm_q4_tc_kernel(const __grid_constant__ QtMaps maps, const float* __restrict__
         const unsigned bar = tc_smem_u32(&full_bar[s]), st = tiles + (unsigned)s * stage_bytes;
         const int k = (step0 + step) * QT_K;
         if (of_w) {
-            tc_mbar_expect_tx(bar, (unsigned)tile.n * (QT_K * 2) + MATS * (QT_CODES + 8 * affine_row));
+            tc_mbar_expect_tx(bar, x_room + MATS * (QT_CODES + 8 * affine_row));
 #pragma unroll
             for (int i = 0; i < MATS; ++i) {
                 const unsigned at = st + x_room + i * (QT_CODES + QT_AFFINE);
@@ -163,9 +160,8 @@ gemm_q4_tc_kernel(const __grid_constant__ QtMaps maps, const float* __restrict__
             }
         }
         if (of_x) {
-            const CUtensorMap* map = tile.n == sh.n ? &maps.x : &maps.x2;
-            tc_tma_load_2d(st, map, k, tile.m0, bar);
-            tc_tma_load_2d(st + (unsigned)tile.n * (TC_BK * 2), map, k + TC_BK, tile.m0, bar);
+            tc_tma_load_2d(st, &maps.x, k, tile.m0, bar);
+            tc_tma_load_2d(st + x_room / 2, &maps.x, k + TC_BK, tile.m0, bar);
         }
     };
     const Tile tile0 = tile_of(0);
@@ -199,11 +195,10 @@ gemm_q4_tc_kernel(const __grid_constant__ QtMaps maps, const float* __restrict__
         int s = 0, place = 0;
         unsigned phase = 0, place_phase = 0;
         bool ok = true;
+        // float32 accumulator, bfloat16 operands, both K-major, N = n, M = 128
+        const unsigned idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(sh.n >> 3) << 17) | (8u << 24);
+        const unsigned x_half = x_room >> 5;   // (in a descriptor's units)
         for (int ti = 0; ok && ti < my_tiles; ++ti) {
-            const Tile tile = tile_of(ti);
-            // float32 accumulator, bfloat16 operands, both K-major, N = n, M = 128
-            const unsigned idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(tile.n >> 3) << 17) | (8u << 24);
-            const unsigned x_half = (unsigned)tile.n * (TC_BK * 2) >> 4;   // (in a descriptor's units)
             ok = !ti || qt_wait(tc_smem_u32(&acc_empty), (unsigned)((ti - 1) & 1));
             for (int i = 0; ok && i < steps; ++i) {
                 ok = qt_wait(tc_smem_u32(&full_bar[s]), phase) && qt_wait(tc_smem_u32(&w_full[place]), place_phase);
@@ -298,7 +293,7 @@ gemm_q4_tc_kernel(const __grid_constant__ QtMaps maps, const float* __restrict__
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
             const unsigned acc = tmem + ((unsigned)(quarter * 32) << 16);
             const Tile tile = tile_of(ti);
-            const int m0 = tile.m0, width = min(tile.n, M - m0), row = tile.w0 + l;
+            const int m0 = tile.m0, width = min(sh.n, M - m0), row = tile.w0 + l;
             const float add = bias && row < N && sh.splits == 1 ? bias[row] : 0.f;
 #pragma unroll 1
             for (int c0 = half * 16; c0 < width; c0 += 32) {
@@ -425,15 +420,13 @@ static int qt_launch(const QtMaps& maps, const float* bias, TO* C, int M, int N,
     return VX_OK;
 }
 
-// With a tile's shape: n a multiple of 16 up to 256 (gated 128), splits up to 8; without splits, the W tiles from full_w on may take tiles of n2 < n
-// rows of x (n2 0: none do).  The other arguments as in vx_gemm_q4.
+// With a tile's shape: n a multiple of 16 up to 256 (gated 128), splits up to 8.  The other arguments as in vx_gemm_q4.
 extern "C" int vx_gemm_q4_tc_shape(const void* x, const void* codes, const void* affine, const void* codes1, const void* affine1, const float* bias,
                                    void* out, int M, int N, int K, int ldx, int ldo, int group, int act, int out_dtype, int w_ready, int n,
-                                   int splits, int full_w, int n2, int* error, cudaStream_t stream) {
+                                   int splits, int* error, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return VX_OK;
-    const int mats = codes1 ? 2 : 1, blocks = (K + 63) / 64, steps = (blocks + 1) / 2, wtiles = (N + 127) / 128;
+    const int mats = codes1 ? 2 : 1, blocks = (K + 63) / 64, steps = (blocks + 1) / 2;
     if (K <= 0 || !error || n < 16 || n > 256 / mats || (n & 15) || splits < 1 || splits > 8 || splits > steps) return VX_ERR_SHAPE;
-    if (n2 && (splits > 1 || n2 < 16 || n2 > n || (n2 & 15) || full_w < 0 || full_w > wtiles)) return VX_ERR_SHAPE;
     if ((group != 32 && group != 64 && group != 128) || K % group || ldx < K || ldo < N) return VX_ERR_SHAPE;
     if (codes1 && (!affine1 || bias || act < 0 || act > VX_ACT_LAST)) return VX_ERR_SHAPE;
     if (out_dtype != VX_BF16 && (out_dtype != VX_F32 || codes1)) return VX_ERR_DTYPE;
@@ -442,8 +435,6 @@ extern "C" int vx_gemm_q4_tc_shape(const void* x, const void* codes, const void*
     sh.n = n;
     sh.steps = (steps + splits - 1) / splits;
     sh.splits = (steps + sh.steps - 1) / sh.steps;   // (no run is empty)
-    sh.full_w = n2 ? full_w : wtiles;
-    sh.n2 = n2 ? n2 : n;
     const int stage = n * (QT_K * 2) + mats * (QT_CODES + QT_AFFINE), stages = QT_ROOM / stage;
     sh.stages = stages > QT_MAX_STAGES ? QT_MAX_STAGES : stages;
     size_t bytes = (size_t)sh.stages * stage;
@@ -457,15 +448,13 @@ extern "C" int vx_gemm_q4_tc_shape(const void* x, const void* codes, const void*
     if (!tc_make_map(&maps.x, x, M, K, ldx, n) || !qt_make_map(&maps.codes[0], codes, wt, words, 2 * Q4_BLOCK_WORDS) ||
         !qt_make_map(&maps.affine[0], affine, wt, pairs, box))
         return VX_ERR_DRIVER;
-    maps.x2 = maps.x;
-    if (sh.n2 != n && !tc_make_map(&maps.x2, x, M, K, ldx, sh.n2)) return VX_ERR_DRIVER;
     maps.codes[1] = maps.codes[0];
     maps.affine[1] = maps.affine[0];
     if (codes1 && (!qt_make_map(&maps.codes[1], codes1, wt, words, 2 * Q4_BLOCK_WORDS) || !qt_make_map(&maps.affine[1], affine1, wt, pairs, box)))
         return VX_ERR_DRIVER;
     static int sm_counts[VX_MAX_DEVICES];
     const int sms = vx_sm_count(sm_counts);
-    const long long tiles = (long long)sh.full_w * ((M + n - 1) / n) + (long long)(wtiles - sh.full_w) * ((M + sh.n2 - 1) / sh.n2);
+    const long long tiles = (long long)((N + 127) / 128) * ((M + n - 1) / n);
     if (tiles > 0x7fffff) return VX_ERR_LIMIT;
     const int teams = sh.splits > 1 ? (int)tiles : (int)(tiles < sms ? tiles : sms);
 #define QT_GO(G_, T_) qt_launch<G_, T_>(maps, bias, (T_*)out, M, N, blocks, ldo, act, group, w_ready, sh, bytes + 1024, teams, error, stream)
@@ -474,16 +463,67 @@ extern "C" int vx_gemm_q4_tc_shape(const void* x, const void* codes, const void*
 #undef QT_GO
 }
 
-// The product with a tile that fits: the arguments as above.
+// Clusters of `blocks` blocks, each of which fills an SM, that run at once (a cluster lies within a group of SMs).
+static int qt_clusters(int blocks, int sms) {
+    static int cache[VX_MAX_DEVICES][9];
+    const int dev = vx_current_device();
+    if (dev < 0) return sms / blocks / 2;
+    int& n = cache[dev][blocks];
+    if (!n) {
+        static bool configured[VX_MAX_DEVICES];
+        auto kernel = gemm_q4_tc_kernel<false, bf16>;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = blocks;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(blocks * sms));
+        cfg.blockDim = dim3(QT_THREADS);
+        cfg.dynamicSmemBytes = 222 * 1024;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        int found = 0;
+        if (vx_configure_smem(kernel, 226 * 1024, configured) != VX_OK || cudaOccupancyMaxActiveClusters(&found, kernel, &cfg) != cudaSuccess || found <= 0) {
+            cudaGetLastError();
+            found = sms / blocks / 2;
+        }
+        n = found;
+    }
+    return n;
+}
+
+// The tile: rows of x (n) and runs of k, the least time by rounds of the SMs.  A step of 128 k takes 0.27 us + 2.1 ns a row of x (gated
+// 0.55 + 3 ns), a tile begins and ends in 4.5 us, and adding the runs' sums takes 0.5 us (four runs: 2) + 17 ns a row.  Measured and so, us, runs
+// 1 / 2 / 4: 32 x 4096 x 4096 14.6, 10.6, 9.6 (15.3, 11.0, 9.7); 128 x 4096 x 4096 19.1, 15.4, 12.4 (21.7, 15.8, 12.9); 64 x 4096 x 12288 42.5,
+// 25.5, 17.6 (43.3, 25.8, 17.2); gated 32 x 9728 x 2560 16.8, whole (17.4).  Three runs, or more clusters than run at once, make some wait
+// for the others: 32 x 6144 x 4096 in two runs 11.8, in three 18.8.
+struct QtPlan { int n, splits; };
+static QtPlan qt_plan(int M, int N, int K, bool gated, int sms) {
+    const int steps = (K + QT_K - 1) / QT_K, wtiles = (N + 127) / 128, most = gated ? 128 : 256;
+    QtPlan best = {};
+    double least = 0;
+    for (int xt = (M + most - 1) / most, tries = 0; tries < 8 && !(best.n && best.n <= 32); ++xt, ++tries) {
+        const int n = ((M + xt - 1) / xt + 15) & ~15;
+        const long long tiles = (long long)wtiles * ((M + n - 1) / n);
+        const double step = gated ? 0.55 + 0.003 * n : 0.27 + 0.0021 * n;
+        for (int splits = 1; splits <= 4; splits *= 2) {
+            if (splits > 1 && (steps < 2 * splits || tiles > qt_clusters(splits, sms))) break;
+            const long long rounds = splits > 1 ? 1 : (tiles + sms - 1) / sms;
+            const double cost = (double)rounds * ((steps + splits - 1) / splits) * step + (splits == 1 ? 0 : (splits == 2 ? 0.5 : 2.0) + 0.017 * n);
+            if (!best.n || cost < least) { best = QtPlan{n, splits}; least = cost; }
+        }
+    }
+    return best;
+}
+
+// The product with that tile: the arguments as above.
 extern "C" int vx_gemm_q4_tc(const void* x, const void* codes, const void* affine, const void* codes1, const void* affine1, const float* bias,
                              void* out, int M, int N, int K, int ldx, int ldo, int group, int act, int out_dtype, int w_ready, int* error,
                              cudaStream_t stream) {
     if (M <= 0 || N <= 0) return VX_OK;
+    if (K <= 0) return VX_ERR_SHAPE;
     static int sm_counts[VX_MAX_DEVICES];
-    const int sms = vx_sm_count(sm_counts), most = codes1 ? 128 : 256, blocks = (K + 63) / 64;
-    const int xt = (M + most - 1) / most, n = ((M + xt - 1) / xt + 15) & ~15, tiles = (N + 127) / 128 * xt;
-    int splits = sms / tiles;
-    if (splits > blocks / 8) splits = blocks / 8;
-    splits = splits < 1 ? 1 : (splits > 8 ? 8 : splits);
-    return vx_gemm_q4_tc_shape(x, codes, affine, codes1, affine1, bias, out, M, N, K, ldx, ldo, group, act, out_dtype, w_ready, n, splits, 0, 0, error, stream);
+    const QtPlan p = qt_plan(M, N, K, codes1 != nullptr, vx_sm_count(sm_counts));
+    return vx_gemm_q4_tc_shape(x, codes, affine, codes1, affine1, bias, out, M, N, K, ldx, ldo, group, act, out_dtype, w_ready, p.n, p.splits, error,
+                               stream);
 }

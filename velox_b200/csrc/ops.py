@@ -197,7 +197,7 @@ def _declare(lib) -> None:
         "vx_quantize_q4": [P, P, P, I, I, c_longlong, I, I, P],
         "vx_dequantize_q4": [P, P, P, I, I, I, P],
         "vx_gemm_q4": [P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, P, P],
-        "vx_gemm_q4_tc_shape": [P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, I, I, P, P],
+        "vx_gemm_q4_tc_shape": [P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, P, P],
     }
     lib.vx_set_pdl_mask.argtypes = [I]
     lib.vx_host_word.argtypes, lib.vx_host_word.restype = [], c_void_p
