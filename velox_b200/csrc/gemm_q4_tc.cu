@@ -46,14 +46,11 @@ struct QtShape {
 };
 struct QtMaps { CUtensorMap x, codes[2], affine[2]; };
 
-__device__ __forceinline__ void qt_st32(unsigned taddr, const unsigned (&r)[32]) {
+__device__ __forceinline__ void qt_st16(unsigned taddr, const unsigned (&r)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n"
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n"
         ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
-        "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
 __device__ __forceinline__ void qt_ld16(unsigned taddr, unsigned (&r)[16]) {
@@ -104,8 +101,11 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
 gemm_q4_tc_kernel(const __grid_constant__ QtMaps maps, const float* __restrict__ bias, TO* __restrict__ C, int M, int N, int blocks, int ldc, int act,
                   int group, int w_ready, const QtShape sh, int* __restrict__ error) {
     constexpr int MATS = GATED ? 2 : 1, PLACES = GATED ? 2 : 4;   // (places: steps whose values there is room for)
+    // A step's products begin when its values are there: gated, half by half, so that the groups that make the two halves do not go in
+    // step with each other, all making values and all waiting.  (Plain, the groups take turns at steps.)
+    constexpr int PARTS = GATED ? 2 : 1;
     extern __shared__ unsigned char qt_raw[];
-    __shared__ __align__(8) unsigned long long full_bar[QT_MAX_STAGES], empty_bar[QT_MAX_STAGES], w_full[PLACES], w_empty[PLACES], acc_full, acc_empty;
+    __shared__ __align__(8) unsigned long long full_bar[QT_MAX_STAGES], empty_bar[QT_MAX_STAGES], w_full[PLACES * PARTS], w_empty[PLACES * PARTS], acc_full[2], acc_empty[2];
     __shared__ unsigned tmem_s;
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int split = sh.splits > 1 ? (int)tp_cluster_rank() : 0;
@@ -117,6 +117,7 @@ gemm_q4_tc_kernel(const __grid_constant__ QtMaps maps, const float* __restrict__
     const int xt = (M + sh.n - 1) / sh.n, total = (N + 127) / 128 * xt;
     const int me = (int)blockIdx.x / sh.splits, teams = (int)gridDim.x / sh.splits;
     const int my_tiles = (total - me + teams - 1) / teams;
+    const int buffers = 2 * MATS * sh.n <= QT_PLACES_AT ? 2 : 1;   // accumulators: two where there is room, so that a tile's epilogue runs under the next one's products
     // (once a tile: divisions.  Once a load they were most of the producer's time.)  Tiles that are worked on at the same time share rows of W.
     struct Tile { int w0, m0; };
     auto tile_of = [&](int ti) {
@@ -129,12 +130,14 @@ gemm_q4_tc_kernel(const __grid_constant__ QtMaps maps, const float* __restrict__
             // the commit of the products that read the stage's x; plain, the warps that make W's values too (see there)
             tc_mbar_init(tc_smem_u32(&empty_bar[s]), GATED ? 1 : 1 + 4 * QT_TEAMS);
         }
-        for (int p = 0; p < PLACES; ++p) {
-            tc_mbar_init(tc_smem_u32(&w_full[p]), 8 * MATS);   // the warps that fill it
-            tc_mbar_init(tc_smem_u32(&w_empty[p]), 1);         // the commit of the products that read it
+        for (int p = 0; p < PLACES * PARTS; ++p) {
+            tc_mbar_init(tc_smem_u32(&w_full[p]), 8);   // the warps that fill it
+            tc_mbar_init(tc_smem_u32(&w_empty[p]), 1);  // the commit of the products that read it
         }
-        tc_mbar_init(tc_smem_u32(&acc_full), 1);
-        tc_mbar_init(tc_smem_u32(&acc_empty), 8);              // the epilogue's warps
+        for (int b = 0; b < 2; ++b) {
+            tc_mbar_init(tc_smem_u32(&acc_full[b]), 1);
+            tc_mbar_init(tc_smem_u32(&acc_empty[b]), 8);   // the epilogue's warps
+        }
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     if (warp == 1) {
@@ -199,25 +202,32 @@ gemm_q4_tc_kernel(const __grid_constant__ QtMaps maps, const float* __restrict__
         const unsigned idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(sh.n >> 3) << 17) | (8u << 24);
         const unsigned x_half = x_room >> 5;   // (in a descriptor's units)
         for (int ti = 0; ok && ti < my_tiles; ++ti) {
-            ok = !ti || qt_wait(tc_smem_u32(&acc_empty), (unsigned)((ti - 1) & 1));
+            const int buf = buffers == 2 ? ti & 1 : 0, use = buffers == 2 ? ti >> 1 : ti;
+            const unsigned d = tmem + (unsigned)(buf * MATS * sh.n);
+            ok = !use || qt_wait(tc_smem_u32(&acc_empty[buf]), (unsigned)((use - 1) & 1));
             for (int i = 0; ok && i < steps; ++i) {
-                ok = qt_wait(tc_smem_u32(&full_bar[s]), phase) && qt_wait(tc_smem_u32(&w_full[place]), place_phase);
-                if (!ok) break;
-                asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                ok = qt_wait(tc_smem_u32(&full_bar[s]), phase);
                 const unsigned xd = tc_desc_lo(tiles + (unsigned)s * stage_bytes), a = tmem + QT_PLACES_AT + (unsigned)(place * MATS * 64);
-                if (tc_elect()) {
 #pragma unroll
-                    for (int m = 0; m < MATS; ++m) {
-                        qt_mma_64(tmem + (unsigned)(m * sh.n), a + m * 64, xd, idesc, i > 0);
-                        qt_mma_64(tmem + (unsigned)(m * sh.n), a + m * 64 + 32, xd + x_half, idesc, 1u);
+                for (int part = 0; part < PARTS; ++part) {
+                    ok = ok && qt_wait(tc_smem_u32(&w_full[place * PARTS + part]), place_phase);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                    if (tc_elect()) {
+#pragma unroll
+                        for (int h = part; h < (PARTS == 2 ? part + 1 : 2); ++h)
+#pragma unroll
+                            for (int m = 0; m < MATS; ++m)
+                                qt_mma_64(d + (unsigned)(m * sh.n), a + m * 64 + h * 32, xd + h * x_half, idesc, h ? 1u : (unsigned)(i > 0));
+                        tc_commit(tc_smem_u32(&w_empty[place * PARTS + part]));
+                        if (part == PARTS - 1) tc_commit(tc_smem_u32(&empty_bar[s]));
                     }
-                    tc_commit(tc_smem_u32(&w_empty[place]));
-                    tc_commit(tc_smem_u32(&empty_bar[s]));
                 }
+                if (!ok) break;
                 if (++place == PLACES) { place = 0; place_phase ^= 1; }
                 if (++s == sh.stages) { s = 0; phase ^= 1; }
             }
-            if (ok && tc_elect()) tc_commit(tc_smem_u32(&acc_full));
+            if (ok && tc_elect()) tc_commit(tc_smem_u32(&acc_full[buf]));
         }
         if (!ok && lane == 0) atomicExch(error, QT_ERR_MMA);
     } else if (warp < QT_EPILOGUE) {
@@ -254,27 +264,34 @@ gemm_q4_tc_kernel(const __grid_constant__ QtMaps maps, const float* __restrict__
         };
         bool ok = i >= all || fetch(i, true);
         for (; ok && i < all; i += STRIDE) {
-            unsigned w[32];
-            const unsigned s0 = q4_scale(a0), b0 = q4_offset(a0), s1 = q4_scale(a1), b1 = q4_offset(a1);
+            // 32 k at a time: the first half's values are on their way to tensor memory while the second's are made
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                unsigned v[4];
-                q4_values(q[t].x, t < 2 ? s0 : s1, t < 2 ? b0 : b1, v);
-                w[8 * t] = v[0]; w[8 * t + 1] = v[1]; w[8 * t + 2] = v[2]; w[8 * t + 3] = v[3];
-                q4_values(q[t].y, t < 2 ? s0 : s1, t < 2 ? b0 : b1, v);
-                w[8 * t + 4] = v[0]; w[8 * t + 5] = v[1]; w[8 * t + 6] = v[2]; w[8 * t + 7] = v[3];
+            for (int h = 0; h < 2; ++h) {
+                const unsigned scale = q4_scale(h ? a1 : a0), offset = q4_offset(h ? a1 : a0);
+                unsigned w[16];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    unsigned v[4];
+                    q4_values(q[2 * h + t].x, scale, offset, v);
+                    w[8 * t] = v[0]; w[8 * t + 1] = v[1]; w[8 * t + 2] = v[2]; w[8 * t + 3] = v[3];
+                    q4_values(q[2 * h + t].y, scale, offset, v);
+                    w[8 * t + 4] = v[0]; w[8 * t + 5] = v[1]; w[8 * t + 6] = v[2]; w[8 * t + 7] = v[3];
+                }
+                if (h == 0) {
+                    ok = qt_wait(tc_smem_u32(&w_empty[place * PARTS + (GATED ? part : 0)]), place_phase);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                }
+                qt_st16(lanes + place * (MATS * 64) + h * 16, w);
             }
-            ok = qt_wait(tc_smem_u32(&w_empty[place]), place_phase);
             if (!ok) break;
-            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-            qt_st32(lanes + place * (MATS * 64), w);
             // The next step's codes while the values are on their way, if they have come.  (Waited for only behind the arrival: the ring may
             // have no stage for them until this step's products have ended.)
             const bool last = i + STRIDE >= all, there = !last && fetch(i + STRIDE, false);
             asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
             __syncwarp();
-            if (lane == 0) qt_arrive(tc_smem_u32(&w_full[place]));
+            if (lane == 0) qt_arrive(tc_smem_u32(&w_full[place * PARTS + (GATED ? part : 0)]));
             if (!last && !there) ok = fetch(i + STRIDE, true);
             place += STRIDE;
             if (place >= PLACES) { place -= PLACES; place_phase ^= 1; }
@@ -286,12 +303,13 @@ gemm_q4_tc_kernel(const __grid_constant__ QtMaps maps, const float* __restrict__
         const bool pairs = !(ldc & 1);
         bool ok = true;
         for (int ti = 0; ti < my_tiles; ++ti) {
+            const int buf = buffers == 2 ? ti & 1 : 0, use = buffers == 2 ? ti >> 1 : ti;
             if (ok) {
-                ok = qt_wait(tc_smem_u32(&acc_full), (unsigned)(ti & 1));
+                ok = qt_wait(tc_smem_u32(&acc_full[buf]), (unsigned)(use & 1));
                 if (!ok && lane == 0) atomicExch(error, QT_ERR_EPILOGUE);
             }
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-            const unsigned acc = tmem + ((unsigned)(quarter * 32) << 16);
+            const unsigned acc = tmem + (unsigned)(buf * MATS * sh.n) + ((unsigned)(quarter * 32) << 16);
             const Tile tile = tile_of(ti);
             const int m0 = tile.m0, width = min(sh.n, M - m0), row = tile.w0 + l;
             const float add = bias && row < N && sh.splits == 1 ? bias[row] : 0.f;
@@ -347,7 +365,7 @@ gemm_q4_tc_kernel(const __grid_constant__ QtMaps maps, const float* __restrict__
             // the accumulator may be overwritten once the epilogue's warps have read it
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
             __syncwarp();
-            if (lane == 0) qt_arrive(tc_smem_u32(&acc_empty));
+            if (lane == 0) qt_arrive(tc_smem_u32(&acc_empty[buf]));
         }
     }
     // All roles meet before the tensor memory goes back; with splits all blocks of the cluster, and all their sums are there.
