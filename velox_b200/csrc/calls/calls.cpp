@@ -323,41 +323,53 @@ PyObject* decode_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
 // A matrix in four bits: its codes, its scales and offsets, its sizes.
 struct Q4 {
     Arg codes, affine;
-    Q4(PyObject* c, PyObject* a) : codes(c), affine(a) {}
+    int rows, depth, group;
+    Q4(PyObject* c, PyObject* a, int rows_, int depth_, int group_) : codes(c), affine(a), rows(rows_), depth(depth_), group(group_) {}
     static int64_t blocks(int64_t depth) { return (depth + 63) / 64; }
     static bool sized(int rows, int depth, int group) {
         return rows > 0 && depth > 0 && (group == 32 || group == 64 || group == 128) && depth % group == 0;
     }
-    bool fine(int rows, int depth, int group, int device) const {
+    bool fine(int device) const {
+        if (!sized(rows, depth, group)) return false;
         const int64_t tiles = ((int64_t)rows + 15) / 16;
         return is(codes, at::kInt) && is16(affine) && codes->is_contiguous() && affine->is_contiguous() && aligned16(*codes) && aligned16(*affine) &&
                codes->numel() == tiles * blocks(depth) * 128 && affine->numel() == tiles * (blocks(depth) * 64 / group) * 32 &&
                codes->get_device() == device && affine->get_device() == device;
     }
+    // from (codes, affine, rows, depth, group)
+    static Q4 of(PyObject* parts, Scalars& sc) {
+        if (!PyTuple_Check(parts) || PyTuple_GET_SIZE(parts) != 5) {
+            sc.bad = true;
+            return Q4(Py_None, Py_None, 0, 0, 0);
+        }
+        return Q4(PyTuple_GET_ITEM(parts, 0), PyTuple_GET_ITEM(parts, 1), sc.i(PyTuple_GET_ITEM(parts, 2)), sc.i(PyTuple_GET_ITEM(parts, 3)),
+                  sc.i(PyTuple_GET_ITEM(parts, 4)));
+    }
 };
 
-// (a, codes, affine, up's codes or None, up's affine or None, bias, rows, depth, group, activation, out dtype, w is ready, the error word's address)
+// (a, the matrix, the up matrix or None, bias, activation, out dtype, w is ready, the error word's address); a matrix: (codes, affine, rows, depth, group)
 PyObject* gemm_q4(PyObject*, PyObject* const* o, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 13) NOT_HERE;
+    if (n != 8) NOT_HERE;
     Arg a(o[0]);
-    Q4 w(o[1], o[2]), up(o[3], o[4]);
-    Optional bias(o[5]);
     Scalars sc;
-    const int N = sc.i(o[6]), K = sc.i(o[7]), group = sc.i(o[8]), act = sc.i(o[9]), ready = sc.i(o[11]);
-    void* const error = sc.p(o[12]);
-    const bool gated = o[3] != Py_None;
-    if (sc.bad || !is16(a) || !THPDtype_Check(o[10]) || !bias.is(at::kFloat) || !Q4::sized(N, K, group)) NOT_HERE;
-    const int device = c10::cuda::current_device();
-    const at::ScalarType kind = ((THPDtype*)o[10])->scalar_type;
-    if (code_of(kind) < 0 || a->dim() != 2 || a->size(1) != K || a->size(0) <= 0 || !small(a->size(0)) || a->get_device() != device || !w.fine(N, K, group, device) ||
-        (gated && !up.fine(N, K, group, device)) || (bias && (bias.a->numel() != N || !bias.a->is_contiguous() || bias.a->get_device() != device)))
+    const bool gated = o[2] != Py_None;
+    const Q4 w = Q4::of(o[1], sc), up = gated ? Q4::of(o[2], sc) : w;
+    Optional bias(o[3]);
+    const int act = sc.i(o[4]), ready = sc.i(o[6]);
+    void* const error = sc.p(o[7]);
+    if (sc.bad || !is16(a) || !THPDtype_Check(o[5]) || !bias.is(at::kFloat)) NOT_HERE;
+    const int device = c10::cuda::current_device(), N = w.rows, K = w.depth;
+    const at::ScalarType kind = ((THPDtype*)o[5])->scalar_type;
+    if (code_of(kind) < 0 || a->dim() != 2 || a->size(1) != K || a->size(0) <= 0 || !small(a->size(0)) || a->get_device() != device || !w.fine(device) ||
+        (gated && (!up.fine(device) || up.rows != N || up.depth != K || up.group != w.group)) ||
+        (bias && (bias.a->numel() != N || !bias.a->is_contiguous() || bias.a->get_device() != device)))
         NOT_HERE;
     const int64_t M = a->size(0), lda = M > 1 ? a->stride(0) : K;
     if (a->stride(1) != 1 || lda % 8 || lda < K || !small(lda) || !aligned16(*a)) NOT_HERE;
     at::Tensor out = fresh(M, N, kind, *a);
     LAUNCH(rc, entry.gemm_q4(a->data_ptr(), w.codes->data_ptr(), w.affine->data_ptr(), gated ? up.codes->data_ptr() : nullptr,
-                             gated ? up.affine->data_ptr() : nullptr, bias.ptr(), out.data_ptr(), (int)M, N, K, (int)lda, N, group, act,
+                             gated ? up.affine->data_ptr() : nullptr, bias.ptr(), out.data_ptr(), (int)M, N, K, (int)lda, N, w.group, act,
                              code_of(kind), ready, error, s));
     return result(rc, std::move(out));
     END_HANDLE_TH_ERRORS
@@ -382,16 +394,15 @@ PyObject* quantize_q4(PyObject*, PyObject* const* o, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// (codes, affine, rows, depth, group)
+// (the matrix): what it stands for
 PyObject* dequantize_q4(PyObject*, PyObject* const* o, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 5) NOT_HERE;
-    Q4 w(o[0], o[1]);
+    if (n != 1) NOT_HERE;
     Scalars sc;
-    const int N = sc.i(o[2]), K = sc.i(o[3]), group = sc.i(o[4]);
-    if (sc.bad || !Q4::sized(N, K, group) || !w.fine(N, K, group, c10::cuda::current_device())) NOT_HERE;
-    at::Tensor out = fresh(N, K, at::kBFloat16, *w.codes);
-    LAUNCH(rc, entry.dequantize_q4(w.codes->data_ptr(), w.affine->data_ptr(), out.data_ptr(), N, K, group, s));
+    const Q4 w = Q4::of(o[0], sc);
+    if (sc.bad || !w.fine(c10::cuda::current_device())) NOT_HERE;
+    at::Tensor out = fresh(w.rows, w.depth, at::kBFloat16, *w.codes);
+    LAUNCH(rc, entry.dequantize_q4(w.codes->data_ptr(), w.affine->data_ptr(), out.data_ptr(), w.rows, w.depth, w.group, s));
     return result(rc, std::move(out));
     END_HANDLE_TH_ERRORS
 }

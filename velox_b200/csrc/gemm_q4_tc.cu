@@ -511,7 +511,8 @@ static int qt_clusters(int blocks, int sms) {
 }
 
 // The tile: rows of x (n) and runs of k, the least time by rounds of the SMs.  A step of 128 k takes 0.27 us + 2.1 ns a row of x (gated
-// 0.55 + 3 ns), a tile begins and ends in 4.5 us, and adding the runs' sums takes 0.5 us (four runs: 2) + 17 ns a row.  Measured and so, us, runs
+// 0.55 + 3 ns), adding the runs' sums 1.2 us (four runs: 1.5) + 17 ns a row, and writing a tile 8 ns a row (gated 25), once, or in every
+// round where there is room for one accumulator only; 4.5 us besides.  Measured and so, us, runs
 // 1 / 2 / 4: 32 x 4096 x 4096 14.6, 10.6, 9.6 (15.3, 11.0, 9.7); 128 x 4096 x 4096 19.1, 15.4, 12.4 (21.7, 15.8, 12.9); 64 x 4096 x 12288 42.5,
 // 25.5, 17.6 (43.3, 25.8, 17.2); gated 32 x 9728 x 2560 16.8, whole (17.4).  Three runs, or more clusters than run at once, make some wait
 // for the others: 32 x 6144 x 4096 in two runs 11.8, in three 18.8.
@@ -520,14 +521,17 @@ static QtPlan qt_plan(int M, int N, int K, bool gated, int sms) {
     const int steps = (K + QT_K - 1) / QT_K, wtiles = (N + 127) / 128, most = gated ? 128 : 256;
     QtPlan best = {};
     double least = 0;
-    for (int xt = (M + most - 1) / most, tries = 0; tries < 8 && !(best.n && best.n <= 32); ++xt, ++tries) {
-        const int n = ((M + xt - 1) / xt + 15) & ~15;
+    for (int rows = most, last = 0; rows >= 16; rows -= 16) {
+        const int xt = (M + rows - 1) / rows, n = ((M + xt - 1) / xt + 15) & ~15;   // (as even as xt tiles can be)
+        if (n == last) continue;
+        last = n;
         const long long tiles = (long long)wtiles * ((M + n - 1) / n);
         const double step = gated ? 0.55 + 0.003 * n : 0.27 + 0.0021 * n;
         for (int splits = 1; splits <= 4; splits *= 2) {
             if (splits > 1 && (steps < 2 * splits || tiles > qt_clusters(splits, sms))) break;
             const long long rounds = splits > 1 ? 1 : (tiles + sms - 1) / sms;
-            const double cost = (double)rounds * ((steps + splits - 1) / splits) * step + (splits == 1 ? 0 : (splits == 2 ? 0.5 : 2.0) + 0.017 * n);
+            const double cost = (double)rounds * ((steps + splits - 1) / splits) * step + (splits == 1 ? 0 : (splits == 2 ? 1.2 : 1.5) + 0.017 * n) +
+                                (gated ? 0.025 : 0.008) * n * (n * (gated ? 4 : 2) > QT_PLACES_AT ? rounds : 1);
             if (!best.n || cost < least) { best = QtPlan{n, splits}; least = cost; }
         }
     }

@@ -1976,7 +1976,7 @@ class Q4Matrix:
     `group` neighbours of a row.  Element (n, k) stands for bfloat16(q s + b), its code q and its group's bfloat16 scale s and offset b.
     Made by `quantize_q4`, or from tensors of that layout: codes int32 [ceil(rows / 16), ceil(depth / 64), 4, 8, 2, 2], affine
     bfloat16 [ceil(rows / 16), groups, 8, 2, 2], both contiguous."""
-    __slots__ = ("codes", "affine", "rows", "depth", "group")
+    __slots__ = ("codes", "affine", "rows", "depth", "group", "parts")
 
     def __init__(self, codes: torch.Tensor, affine: torch.Tensor, rows: int, depth: int, group: int):
         tiles, blocks, groups = _q4_sizes(rows, depth, group)
@@ -1986,13 +1986,13 @@ class Q4Matrix:
               "Q4Matrix: scales and offsets must be contiguous bfloat16 %s for [%d, %d] in groups of %d" % ((tiles, groups, 8, 2, 2), rows, depth, group))
         _need(codes.device == affine.device, "Q4Matrix: codes on %s, scales and offsets on %s" % (codes.device, affine.device))
         _need(codes.data_ptr() % 16 == 0 and affine.data_ptr() % 16 == 0, "Q4Matrix: 16-byte aligned tensors")
-        self.codes, self.affine, self.rows, self.depth, self.group = codes, affine, int(rows), int(depth), int(group)
+        self.codes, self.affine, self.rows, self.depth, self.group = self.parts = (codes, affine, int(rows), int(depth), int(group))
 
     @classmethod
     def _of(cls, codes, affine, rows, depth, group):
         """(Tensors that a kernel has just laid out.)"""
         m = cls.__new__(cls)
-        m.codes, m.affine, m.rows, m.depth, m.group = codes, affine, rows, depth, group
+        m.codes, m.affine, m.rows, m.depth, m.group = m.parts = (codes, affine, rows, depth, group)
         return m
 
     @property
@@ -2048,7 +2048,7 @@ def quantize_q4(w: torch.Tensor, group: int = 64) -> Q4Matrix:
 def dequantize_q4(w: Q4Matrix) -> torch.Tensor:
     """The bfloat16 matrix that `w` stands for: what the products multiply with."""
     if w.codes.is_cuda:
-        out = (_CALLS or _calls()).dequantize_q4(w.codes, w.affine, w.rows, w.depth, w.group)
+        out = (_CALLS or _calls()).dequantize_q4(w.parts)
         if out is not None:
             return _called(out, "dequantize_q4")
     _dev(w.codes, w.affine)
@@ -2060,15 +2060,16 @@ def dequantize_q4(w: Q4Matrix) -> torch.Tensor:
     return out
 
 
+def _q4_called(out, what: str):
+    """What the call module gave for a product (not None), its launch counted."""
+    global _BOUNDED_WAIT_LAUNCHES
+    out = _called(out, what)
+    if len(out) > Q4_FEW_ROWS:
+        _BOUNDED_WAIT_LAUNCHES += 1
+    return out
+
+
 def _q4_product(what: str, a: torch.Tensor, w: Q4Matrix, up: Optional[Q4Matrix], bias, out_dtype, act: int, w_ready: bool) -> torch.Tensor:
-    if a.is_cuda:
-        out = (_CALLS or _calls()).gemm_q4(a, w.codes, w.affine, up.codes if up is not None else None, up.affine if up is not None else None,
-                                           bias, w.rows, w.depth, w.group, act, out_dtype, 1 if w_ready else 0, _error_address(a.device))
-        if out is not None:
-            out = _called(out, what)
-            if out.shape[0] > Q4_FEW_ROWS:
-                note_bounded_wait()
-            return out
     _dev(a, w.codes, w.affine, bias)
     _need(a.dtype == torch.bfloat16 and a.dim() == 2 and a.shape[1] == w.depth, "%s: bfloat16 a [M, %d]" % (what, w.depth))
     m, k = a.shape
@@ -2095,12 +2096,20 @@ def gemm_q4(a: torch.Tensor, w: Q4Matrix, bias: Optional[torch.Tensor] = None, o
             w_ready: bool = False) -> torch.Tensor:
     """a [M, K] (bfloat16) times the matrix that `w` [N, K] stands for, transposed (+ float32 `bias` [N]); float32 sums, rounded once to
     `out_dtype` (bfloat16 or float32).  `w_ready`: see `gemm_nt_simt`."""
+    if a.is_cuda:
+        out = (_CALLS or _calls()).gemm_q4(a, w.parts, None, bias, 0, out_dtype or torch.bfloat16, w_ready, _error_address(a.device))
+        if out is not None:
+            return _q4_called(out, "gemm_q4")
     return _q4_product("gemm_q4", a, w, None, bias, out_dtype or torch.bfloat16, 0, w_ready)
 
 
 def gated_q4(a: torch.Tensor, gate: Q4Matrix, up: Q4Matrix, activation: str = "silu", w_ready: bool = False) -> torch.Tensor:
     """act(a Wg^T) * (a Wu^T) in one kernel, [M, N] bfloat16: both projections of a gated feed-forward with matrices in four bits of one
     shape and group; activation and product on the float32 sums, rounded once.  `w_ready`: see `gemm_nt_simt`."""
+    if a.is_cuda and activation in ACTIVATIONS:
+        out = (_CALLS or _calls()).gemm_q4(a, gate.parts, up.parts, None, ACTIVATIONS[activation], torch.bfloat16, w_ready, _error_address(a.device))
+        if out is not None:
+            return _q4_called(out, "gated_q4")
     _need(activation in ACTIVATIONS, "gated_q4: unknown activation %r" % (activation,))
     _need(gate.shape == up.shape and gate.group == up.group and gate.device == up.device,
           "gated_q4: gate %s and up %s of one shape, group and device" % (gate.shape, up.shape))
