@@ -128,6 +128,21 @@ gemm_q4_kernel(const bf16* __restrict__ x, const Q4Pair w, const float* __restri
 #pragma unroll
     for (int j = 0; j < NT; ++j) xr[j] = x + (size_t)min(r + 8 * j, M - 1) * ldx + lo * 64 + t * 16;
     const bool cut = (K & 63) && lo + mine == blocks;   // the warp's last block reaches beyond K: x counts as 0 there (K is a multiple of the group)
+    // block `at` from where the rows are; `last`: the tile's last block, from there
+    auto fetch_x = [&](uint4 (&v)[NT][2], int at, int last) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            if (GROUP == 32 && cut && at == last && t >= 2) {
+                v[j][0] = v[j][1] = make_uint4(0u, 0u, 0u, 0u);
+            } else {
+                v[j][0] = q4_x16(xr[j] + at * 64);
+                v[j][1] = q4_x16(xr[j] + at * 64 + 8);
+            }
+        }
+    };
+    constexpr bool X_AHEAD = NT <= 2;   // x of the next block is asked for before a block's products (with four tiles of columns the registers are short)
+    uint4 xn[NT][2];
+    if (X_AHEAD && mine > 0) fetch_x(xn, 0, mine - 1);
     const unsigned own = (t * 8 + r) * 16, own_affine = Step::codes + r * 8 + (GROUP == 32 ? (t >> 1) * 64 : 0);
     unsigned at = ring;
     const int block_tiles = (units - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
@@ -139,14 +154,15 @@ gemm_q4_kernel(const bf16* __restrict__ x, const Q4Pair w, const float* __restri
             __syncwarp();
             auto block = [&](int b) {
                 uint4 xv[NT][2];
+                if (X_AHEAD) {
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    if (GROUP == 32 && cut && b == left - 1 && t >= 2) {
-                        xv[j][0] = xv[j][1] = make_uint4(0u, 0u, 0u, 0u);
-                    } else {
-                        xv[j][0] = q4_x16(xr[j] + b * 64);
-                        xv[j][1] = q4_x16(xr[j] + b * 64 + 8);
-                    }
+                    for (int j = 0; j < NT; ++j) { xv[j][0] = xn[j][0]; xv[j][1] = xn[j][1]; }
+                    // the next block's: of this step, the next, or the next tile's first
+                    const bool more = b + 1 < BLOCKS && (left >= BLOCKS || b + 1 < left);
+                    const int at = more ? b + 1 : (left > BLOCKS ? BLOCKS : left - mine);
+                    fetch_x(xn, at, left - 1);
+                } else {
+                    fetch_x(xv, b, left - 1);
                 }
 #pragma unroll
                 for (int i = 0; i < MATS; ++i) {
