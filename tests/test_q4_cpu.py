@@ -49,6 +49,16 @@ def test_the_entry_points_refuse_before_they_launch():
                          (dict(codes1=A, affine1=A, dtype=0), DTYPE)]:
         assert product(**change) == code, change
 
+    def tiled(x=A, codes=A, affine=A, codes1=None, affine1=None, bias=None, out=A, m=40, n=32, k=512, ldx=512, ldo=32, group=64, act=0, dtype=1, columns=48,
+              splits=1, error=A):
+        return lib.vx_gemm_q4_tc_shape(x, codes, affine, codes1, affine1, bias, out, m, n, k, ldx, ldo, group, act, dtype, 0, columns, splits, error, None)
+    assert tiled(m=0) == 0 and tiled(n=0) == 0
+    for change, code in [(dict(columns=8), SHAPE), (dict(columns=40), SHAPE), (dict(columns=272), SHAPE), (dict(columns=144, codes1=A, affine1=A), SHAPE),
+                         (dict(splits=0), SHAPE), (dict(splits=9), SHAPE), (dict(splits=5), SHAPE), (dict(error=None), SHAPE), (dict(k=480), SHAPE),
+                         (dict(ldx=504), SHAPE), (dict(ldo=16), SHAPE), (dict(codes1=A), SHAPE), (dict(codes1=A, affine1=A, dtype=0), DTYPE),
+                         (dict(dtype=3), DTYPE), (dict(ldx=516), ALIGN), (dict(codes=A + 8), ALIGN)]:
+        assert tiled(**change) == code, change
+
     def made(w=A, codes=A, affine=A, n=32, k=128, ldw=128, group=64, dtype=1):
         return lib.vx_quantize_q4(w, codes, affine, n, k, ldw, group, dtype, None)
     assert made(n=0) == 0

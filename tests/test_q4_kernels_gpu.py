@@ -88,7 +88,10 @@ def test_quantize_rows_of_a_wider_matrix():
 SIZES = [(1, 16, 64, 64), (1, 2048, 2048, 64), (2, 1, 32, 32), (3, 17, 96, 32), (5, 1000, 1056, 32), (8, 4096, 128, 128), (7, 40, 5120, 128),
          (8, 333, 4096, 64), (9, 100, 256, 64), (16, 130, 1024, 128), (17, 250, 2080, 32), (33, 129, 640, 64), (64, 512, 512, 64),
          (65, 1003, 1056, 32), (127, 256, 1984, 64), (128, 128, 4224, 128), (129, 200, 320, 64), (200, 2048, 2048, 64), (257, 144, 384, 128),
-         (300, 15, 96, 32), (513, 700, 704, 64), (1025, 272, 256, 64)]
+         (300, 15, 96, 32), (513, 700, 704, 64), (1025, 272, 256, 64),
+         # matrices of many rows: blocks that form several tiles, two at a time (an odd number of them), by four warps
+         (8, 5000, 96, 32), (3, 7201, 96, 32), (8, 7216, 576, 64), (1, 38000, 64, 64), (5, 37905, 224, 32), (12, 14401, 128, 128), (24, 7300, 160, 32),
+         (32, 2000, 1024, 64), (20, 38016, 128, 64), (300, 4096, 512, 64), (700, 9001, 128, 128)]
 
 
 @pytest.mark.parametrize("m,n,k,group", SIZES)
@@ -112,6 +115,89 @@ def test_gated(m, n, k, group):
     got = ops.gated_q4(x, gate, up, name)
     want, bound = q4.gated(x64, g64, u64, name)
     q4.close(got, want, bound, torch.bfloat16)
+    ops.check_device_errors()
+
+
+@pytest.mark.parametrize("m,n,k,group", [(100, 300, 1056, 32), (270, 520, 1024, 128), (40, 2100, 640, 64)])
+@pytest.mark.parametrize("columns", [16, 48, 112, 128, 256])
+@pytest.mark.parametrize("splits", [1, 2, 3, 4, 8])
+def test_tiles_of_the_tensor_core_product(m, n, k, group, columns, splits):
+    """Every shape of a tile that the entry point takes, not only those that the sizes choose."""
+    if splits > (k + 127) // 128:
+        pytest.skip("more runs than steps are refused")
+    (w, w64), (up, u64) = made(n, k, group, 3), made(n, k, group, 4)
+    x, x64 = rows_of(m, k, 5)
+    shape, error = ops.library().vx_gemm_q4_tc_shape, ops._error_address(x.device)
+    out = torch.full((m, n), float("nan"), device="cuda")
+    assert shape(x.data_ptr(), w.codes.data_ptr(), w.affine.data_ptr(), None, None, None, out.data_ptr(), m, n, k, k, n, group, 0, 0, 0, columns, splits,
+                 error, ops._stream()) == 0
+    q4.close(out, x64 @ w64.T, q4.sum_bound(x64, w64), torch.float32)
+    if columns <= 128:
+        out = torch.full((m, n), float("nan"), device="cuda", dtype=torch.bfloat16)
+        assert shape(x.data_ptr(), w.codes.data_ptr(), w.affine.data_ptr(), up.codes.data_ptr(), up.affine.data_ptr(), None, out.data_ptr(), m, n, k, k, n,
+                     group, ops.ACTIVATIONS["silu"], 1, 1, columns, splits, error, ops._stream()) == 0
+        q4.close(out, *q4.gated(x64, w64, u64, "silu"), torch.bfloat16)
+    ops.check_device_errors()
+
+
+@pytest.mark.parametrize("m", [2, 16, 40])
+def test_rows_behind_the_result_stay_as_they_were(m):
+    """Odd numbers of columns, a result inside a wider tensor: nothing beside it is written."""
+    n, k = 131, 192
+    w, w64 = made(n, k, 64, 3)
+    x, x64 = rows_of(m, k, 5)
+    wide = torch.full((m + 2, n + 5), 7.0, device="cuda")
+    inner = wide[1:m + 1, 2:n + 2]
+    assert ops.library().vx_gemm_q4(x.data_ptr(), w.codes.data_ptr(), w.affine.data_ptr(), None, None, None, inner.data_ptr(), m, n, k, k, n + 5, 64, 0, 0, 0,
+                                    ops._error_address(x.device), ops._stream()) == 0
+    q4.close(inner, x64 @ w64.T, q4.sum_bound(x64, w64), torch.float32)
+    wide[1:m + 1, 2:n + 2] = 7.0
+    assert bool((wide == 7.0).all())
+
+
+def test_two_streams_at_once():
+    """Both kernels side by side with themselves: nothing is shared."""
+    w, _ = made(2048, 2048, 64, 1)
+    up, _ = made(2048, 2048, 64, 2)
+    xs = [rows_of(m, 2048, m)[0] for m in (4, 90)]
+    want = [(ops.gemm_q4(x, w, None, torch.float32), ops.gated_q4(x, w, up)) for x in xs]
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(10):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append([(ops.gemm_q4(x, w, None, torch.float32), ops.gated_q4(x, w, up)) for x in xs])
+    torch.cuda.synchronize()
+    for g in got:
+        for (a, b), (c, d) in zip(g, want):
+            assert torch.equal(a, c) and torch.equal(b, d)
+    ops.check_device_errors()
+
+
+def test_offsets_beyond_32_bits():
+    """1.2 million rows of 4,096: codes, dense values and results beyond 2^31 bytes and elements; the last rows are those of a small matrix."""
+    n, k, tail = 1200000, 4096, 160
+    codes = torch.zeros(n // 16, k // 64, 4, 8, 2, 2, dtype=torch.int32, device="cuda")
+    affine = torch.zeros(n // 16, k // 64, 8, 2, 2, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    codes[-tail // 16:] = torch.randint(-2 ** 31, 2 ** 31 - 1, codes[-tail // 16:].shape, dtype=torch.int32, device="cuda", generator=g)
+    affine[-tail // 16:] = (torch.rand(affine[-tail // 16:].shape, device="cuda", generator=g) * 0.01).to(torch.bfloat16)
+    big = ops.Q4Matrix(codes, affine, n, k, 64)
+    small = ops.Q4Matrix(codes[-tail // 16:].clone(), affine[-tail // 16:].clone(), tail, k, 64)
+    w64 = q4.matrix(*q4.unpack(small), 64)
+    for m in (1, 40):
+        x, x64 = rows_of(m, k, m)
+        got = ops.gemm_q4(x, big, None, torch.float32)
+        q4.close(got[:, -tail:], x64 @ w64.T, q4.sum_bound(x64, w64), torch.float32)
+        assert float(got[:, :-tail].abs().max()) == 0.0
+        del got
+    dense = ops.dequantize_q4(big)
+    assert np.array_equal(dense[-tail:].double().cpu().numpy(), w64) and float(dense[:-tail].abs().max()) == 0.0
+    del big, codes, affine
+    again = ops.quantize_q4(dense, 64)
+    want = ops.quantize_q4(dense[-tail:], 64)
+    assert torch.equal(again.codes[-tail // 16:], want.codes) and torch.equal(again.affine[-tail // 16:], want.affine)
     ops.check_device_errors()
 
 
