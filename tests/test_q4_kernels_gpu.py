@@ -211,6 +211,33 @@ def test_every_activation(m, name):
     q4.close(ops.gated_q4(x, gate, up, name), want, bound, torch.bfloat16)
 
 
+def odd_matrix(n, k, group, seed):
+    """Scales and offsets of every size and sign: zero, subnormal, at both ends of those that are raised by 2^133, large; mixed within a row,
+    a tile and a warp."""
+    g = torch.Generator().manual_seed(seed)
+    codes = torch.randint(-2 ** 31, 2 ** 31 - 1, (-(-n // 16), -(-k // 64), 4, 8, 2, 2), generator=g, dtype=torch.int32)
+    bits = torch.tensor([0x0000, 0x0001, 0x007f, 0x0080, 0x00ff, 0x3c00, 0x3cff, 0x3d00, 0x3d01, 0x3f80, 0x4300, 0x8000, 0xbc00, 0xbf80], dtype=torch.int32)
+    shape = (-(-n // 16), -(-k // 64) * 64 // group, 8, 2, 2)
+    affine = bits[torch.randint(0, len(bits), shape, generator=g)]
+    affine[..., 1] = bits[torch.randint(5, len(bits), shape[:-1], generator=g)]
+    plain = torch.rand(shape[:2], generator=g) < 0.5     # half of the groups of a tile: scales as trained matrices have them
+    affine[..., 0][plain] = 0x3c10
+    return ops.Q4Matrix(codes.cuda(), affine.to(torch.int16).view(torch.bfloat16).cuda(), n, k, group)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m,n,k", [(1, 64, 512), (8, 7300, 384), (13, 100, 1152), (30, 50, 640), (70, 200, 896), (5, 38000, 256)])
+def test_scales_and_offsets_of_every_size(m, n, k, group):
+    w, up = odd_matrix(n, k, group, m), odd_matrix(n, k, group, m + 1)
+    w64, u64 = (q4.matrix(*q4.unpack(v), group) for v in (w, up))
+    assert np.array_equal(ops.dequantize_q4(w).double().cpu().numpy(), w64)
+    x, x64 = rows_of(m, k, n)
+    q4.close(ops.gemm_q4(x, w, None, torch.float32), x64 @ w64.T, q4.sum_bound(x64, w64), torch.float32)
+    want, bound = q4.gated(x64, w64, u64, "relu")
+    q4.close(ops.gated_q4(x, w, up, "relu"), want, bound, torch.bfloat16)
+    ops.check_device_errors()
+
+
 def test_product_is_that_of_the_dense_matrix():
     """The same matrix, dense and in four bits, through the engine's products: float32 sums of the same terms."""
     w, w64 = made(256, 512, 64, 9)

@@ -1,12 +1,19 @@
 // out[M,N] = x[M,K] W^T (+ bias) and out[M,N] = act(x Wg^T) * (x Wu^T) with matrices held in four bits (q4.cuh), for a few rows: the
-// products of a decode step, where the whole cost is reading codes, scales and offsets once.
+// products of a decode step, whose floor is reading codes, scales and offsets once.
 //
-// As in the bfloat16 product of a few rows, out^T = W x^T on mma.sync.m16n8k16: 16 rows of W fill the tile's 16-row side, up to 8 rows of x its
-// 8-column side.  A block owns the 16 rows of one row of code blocks (gated: those of the gate's and those of the up matrix, so that
-// both sums of a feature meet in it) and the whole of K; its warps take the 64-wide code blocks in turn.  A lane's 16 bytes of a code block are
-// its fragments of four products; it makes them bfloat16 in registers and nothing passes through shared memory.  k is permuted
-// the same way for x, of which a lane reads 32 neighbouring bytes of a row.  The warps' partial tiles are added in shared memory in warp
-// order: the same result on every run, and a row's result does not depend on the rows beside it.
+// As in the bfloat16 product of a few rows, out^T = W x^T on mma.sync.m16n8k16: 16 rows of W fill the instruction's 16-row side, 8 rows of x its
+// 8-column side (NT such tiles of columns for up to 32 rows).  A block forms 16 rows of W at a time, or 32, for which x is read once (gated: 16
+// gate rows and their up rows, so that both sums of a feature meet in it), over the whole of K: its warps have a run of code blocks each.  A
+// warp's steps of four code blocks come by cp.async into a ring of its own, two ahead and across tiles; a lane's 16 bytes of a code block are its
+// fragments of four products, which it makes bfloat16 in registers.  (Through registers alone the loads share what the warp waits on with
+// those of x, and every block waited for memory.)  k is permuted the same way for x, of which a lane reads 32 neighbouring bytes of a
+// row, a code block ahead, through L1.  The warps' sums are added in shared memory in warp order: the same result on every run, and a row's
+// result does not depend on the rows beside it.
+//
+// What bounds it: instructions.  Eight weights take 15 (three shifts, four three-input logic operations, eight packed multiply-adds, two of
+// which a pipe takes every four cycles), and all of a code block 87 to 94 warp instructions with its loads, products and share of a tile's end, against
+// some 90 cycles that its bytes take at the copy rate.  us, and of the copy rate of 6,549 GB/s: gated 12288 x 4096 1 row 14.9, 58 %; gated 17408 x 5120
+// 8 rows 25.4, 61 %; 151936 x 2560 4 rows to float32 48.6, 69 %; 4096 x 12288 1 row 9.1, 48 %.
 #include "q4.cuh"
 
 __device__ __forceinline__ unsigned q4_smem(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
@@ -172,8 +179,8 @@ gemm_q4_kernel(const bf16* __restrict__ x, const Q4Pair w, const float* __restri
 #pragma unroll
                     for (int word = 0; word < 2; ++word) {
                         unsigned w0[4], w1[4];
-                        q4_values(word ? q.y : q.x, s0, b0, w0);
-                        q4_values(word ? q.w : q.z, s1, b1, w1);
+                        q4_values<false>(word ? q.y : q.x, s0, b0, w0);
+                        q4_values<false>(word ? q.w : q.z, s1, b1, w1);
 #pragma unroll
                         for (int j = 0; j < NT; ++j) {
                             q4_mma(acc[i][j], w0[0], w1[0], w0[1], w1[1], xv[j][word].x, xv[j][word].y);
@@ -255,6 +262,11 @@ template <bool GATED, typename TO, int GROUP, int NT>
 static int q4_launch(const bf16* x, const Q4Pair& w, const float* bias, TO* out, int M, int N, int K, int ldx, int ldo, int act,
                      int w_ready, cudaStream_t stream) {
     const int tiles = (N + 15) / 16, sms = q4_sms();
+    // Eight warps a tile, two blocks an SM; three where that lets all tiles be worked on at once; two tiles at a time where there are more; and
+    // four warps by four blocks where there are so many that a tile's end, which all of a block's warps wait for, counts more than a tile's length.
+    // us, this way and the next best: 1 row 4096 x 4096 4.1 (two tiles 4.1, three blocks 4.8); 6144 x 4096 5.2 (two blocks 6.8, two tiles 5.9); 8 rows 7168 x
+    // 5120 two tiles 8.3 (one 8.7); 4 rows 151936 x 2560 49.8 (eight warps 55.0, one tile 53.2).  Gated: 1 row 12288 x 4096 15.5 (four warps 16.9), 9728 x
+    // 2560 10.0 (10.8), 8 rows 17408 x 5120 four warps 26.2 (eight 28.0).
 #define Q4_GO(F_, W_, P_) return q4_go<F_, TO, GROUP, NT, W_, 4, 2, P_>(x, w, bias, out, M, N, K, ldx, ldo, act, w_ready, stream)
     if constexpr (GATED) {
         if (tiles > 6 * sms) Q4_GO(Q4_GATED, 4, 4);

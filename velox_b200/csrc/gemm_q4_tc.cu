@@ -96,6 +96,19 @@ __device__ __forceinline__ void qt_mma_64(unsigned d, unsigned a, unsigned b_lo,
                      ::"r"(d), "r"(a + 8 * k), "r"(b_lo + 2 * k), "r"(idesc), "r"(k ? 1u : add), "r"(TC_DESC_HI) : "memory");
 }
 
+// 32 codes of a row to 16 pairs of values.
+template <bool SMALL>
+__device__ __forceinline__ void qt_values(uint2 first, uint2 second, unsigned affine, unsigned (&w)[16]) {
+    const unsigned scale = SMALL ? q4_raised(q4_scale(affine)) : q4_scale(affine), offset = q4_offset(affine);
+    const unsigned words[4] = {first.x, first.y, second.x, second.y};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        unsigned v[4];
+        q4_values<SMALL>(words[i], scale, offset, v);
+        w[4 * i] = v[0]; w[4 * i + 1] = v[1]; w[4 * i + 2] = v[2]; w[4 * i + 3] = v[3];
+    }
+}
+
 template <bool GATED, typename TO>
 __global__ void __launch_bounds__(QT_THREADS, 1)
 gemm_q4_tc_kernel(const __grid_constant__ QtMaps maps, const float* __restrict__ bias, TO* __restrict__ C, int M, int N, int blocks, int ldc, int act,
@@ -267,16 +280,10 @@ gemm_q4_tc_kernel(const __grid_constant__ QtMaps maps, const float* __restrict__
             // 32 k at a time: the first half's values are on their way to tensor memory while the second's are made
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const unsigned scale = q4_scale(h ? a1 : a0), offset = q4_offset(h ? a1 : a0);
+                const unsigned pair = h ? a1 : a0;
                 unsigned w[16];
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    unsigned v[4];
-                    q4_values(q[2 * h + t].x, scale, offset, v);
-                    w[8 * t] = v[0]; w[8 * t + 1] = v[1]; w[8 * t + 2] = v[2]; w[8 * t + 3] = v[3];
-                    q4_values(q[2 * h + t].y, scale, offset, v);
-                    w[8 * t + 4] = v[0]; w[8 * t + 5] = v[1]; w[8 * t + 6] = v[2]; w[8 * t + 7] = v[3];
-                }
+                if (__all_sync(0xffffffffu, q4_small(pair))) qt_values<true>(q[2 * h], q[2 * h + 1], pair, w);
+                else qt_values<false>(q[2 * h], q[2 * h + 1], pair, w);
                 if (h == 0) {
                     ok = qt_wait(tc_smem_u32(&w_empty[place * PARTS + (GATED ? part : 0)]), place_phase);
                     if (!ok) break;

@@ -169,7 +169,7 @@ dequantize_q4_kernel(const unsigned* __restrict__ codes, const unsigned* __restr
 #pragma unroll
             for (int word = 0; word < 2; ++word) {
                 unsigned w[4];
-                q4_values(words[2 * half + word], s, b, w);
+                q4_values<false>(words[2 * half + word], s, b, w);
                 __stcs(reinterpret_cast<uint4*>(W + row * K + k) + word, make_uint4(w[0], w[1], w[2], w[3]));
             }
         }
