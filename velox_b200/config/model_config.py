@@ -107,8 +107,8 @@ class Qwen3Config(ModelConfig):
     model_type: ClassVar[str] = "qwen3"
     # the reference reads 4-bit checkpoints through these (src/paged/qwen3.rs:51-59)
     unsupported_keys: ClassVar[Dict[str, str]] = {
-        "quantization": "quantized weights are not supported; the engine holds bfloat16 or float32",
-        "quantization_config": "quantized weights are not supported; the engine holds bfloat16 or float32",
+        "quantization": "quantized weights are not supported in a checkpoint; the engine makes its own of a dense one (weight_bits)",
+        "quantization_config": "quantized weights are not supported in a checkpoint; the engine makes its own of a dense one (weight_bits)",
     }
 
     vocab_size: int = _field(int)
