@@ -91,7 +91,9 @@ SIZES = [(1, 16, 64, 64), (1, 2048, 2048, 64), (2, 1, 32, 32), (3, 17, 96, 32), 
          (300, 15, 96, 32), (513, 700, 704, 64), (1025, 272, 256, 64),
          # matrices of many rows: blocks that form several tiles, two at a time (an odd number of them), by four warps
          (8, 5000, 96, 32), (3, 7201, 96, 32), (8, 7216, 576, 64), (1, 38000, 64, 64), (5, 37905, 224, 32), (12, 14401, 128, 128), (24, 7300, 160, 32),
-         (32, 2000, 1024, 64), (20, 38016, 128, 64), (300, 4096, 512, 64), (700, 9001, 128, 128)]
+         (32, 2000, 1024, 64), (20, 38016, 128, 64), (300, 4096, 512, 64), (700, 9001, 128, 128),
+         # depths below a step, a single row of W, very many rows of x
+         (40, 100, 32, 32), (33, 16, 64, 64), (1000, 30, 64, 32), (17, 1, 128, 128), (70001, 48, 64, 64)]
 
 
 @pytest.mark.parametrize("m,n,k,group", SIZES)
