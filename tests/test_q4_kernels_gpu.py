@@ -157,6 +157,29 @@ def test_rows_behind_the_result_stay_as_they_were(m):
     assert bool((wide == 7.0).all())
 
 
+@pytest.mark.parametrize("m", [2, 40, 150])
+@pytest.mark.parametrize("n", [131, 132])
+@pytest.mark.parametrize("left,gap", [(2, 5), (1, 4), (2, 4), (1, 5)])
+def test_bfloat16_results_inside_a_wider_tensor(m, n, left, gap):
+    """Odd and even widths, distances and first elements: right inside, and nothing beside it is written."""
+    k = 192
+    (w, w64), (up, u64) = made(n, k, 64, 3), made(n, k, 64, 4)
+    x, x64 = rows_of(m, k, 5)
+    lib, error = ops.library(), ops._error_address(x.device)
+    for second in (None, up):
+        wide = torch.full((m + 2, n + gap), 7.0, device="cuda", dtype=torch.bfloat16)
+        inner = wide[1:m + 1, left:n + left]
+        assert lib.vx_gemm_q4(x.data_ptr(), w.codes.data_ptr(), w.affine.data_ptr(), second and second.codes.data_ptr(), second and second.affine.data_ptr(),
+                              None, inner.data_ptr(), m, n, k, k, n + gap, 64, ops.ACTIVATIONS["silu"], 1, 0, error, ops._stream()) == 0
+        if second:
+            q4.close(inner, *q4.gated(x64, w64, u64, "silu"), torch.bfloat16)
+        else:
+            q4.close(inner, x64 @ w64.T, q4.sum_bound(x64, w64), torch.bfloat16)
+        wide[1:m + 1, left:n + left] = 7.0
+        assert bool((wide == 7.0).all())
+    ops.check_device_errors()
+
+
 def test_two_streams_at_once():
     """Both kernels side by side with themselves: nothing is shared."""
     w, _ = made(2048, 2048, 64, 1)

@@ -307,7 +307,7 @@ gemm_q4_tc_kernel(const __grid_constant__ QtMaps maps, const float* __restrict__
     } else {
         const int quarter = warp & 3, half = (warp - QT_EPILOGUE) >> 2;
         const int l = quarter * 32 + lane;   // this thread's row of the block's 128 rows of W
-        const bool pairs = !(ldc & 1);
+        const bool pairs = !((ldc | N) & 1) && !(reinterpret_cast<uintptr_t>(C) & 3);   // (an odd N's last row has no neighbour to be stored with)
         bool ok = true;
         for (int ti = 0; ti < my_tiles; ++ti) {
             const int buf = buffers == 2 ? ti & 1 : 0, use = buffers == 2 ? ti >> 1 : ti;
