@@ -69,6 +69,24 @@ def test_the_entry_points_refuse_before_they_launch():
     assert lib.vx_dequantize_q4(A, A, A, 32, 96, 64, None) == SHAPE and lib.vx_dequantize_q4(A, A, A + 2, 32, 128, 64, None) == ALIGN
 
 
+def test_the_entry_points_refuse_sizes_beyond_their_arithmetic():
+    """Sizes that cannot be rounded up to a tile within 31 bits, and on the tensor cores depths beyond 2^24."""
+    lib = ops.library()
+    A, most, deep = 1 << 20, 2 ** 31 - 1, 2 ** 31 - 128
+
+    def product(m, n, k, codes1=None):
+        return lib.vx_gemm_q4(A, A, A, codes1, codes1, None, A, m, n, k, k, n, 128, 0, 1, 0, A, None)
+    for codes1 in (None, A):
+        assert product(1, most, 128, codes1) == LIMIT and product(most, 128, 128, codes1) == LIMIT and product(most, most, 128, codes1) == LIMIT
+        assert product(1, 16, deep, codes1) == LIMIT and product(40, 128, deep, codes1) == LIMIT
+        assert product(40, 128, (1 << 24) + 128, codes1) == LIMIT
+    for m, n, k in [(40, most, 128), (most, 128, 128), (40, 128, deep), (40, 128, (1 << 24) + 128)]:
+        assert lib.vx_gemm_q4_tc_shape(A, A, A, None, None, None, A, m, n, k, k, n, 128, 0, 1, 0, 48, 1, A, None) == LIMIT
+    for n, k in [(most, 128), (16, deep)]:
+        assert lib.vx_quantize_q4(A, A, A, n, k, k, 128, 1, None) == LIMIT
+        assert lib.vx_dequantize_q4(A, A, A, n, k, 128, None) == LIMIT
+
+
 def test_engine_settings():
     from velox_b200 import EngineConfig
     cfg = EngineConfig(weight_bits=4, weight_group=128, head_bits=4)

@@ -298,6 +298,7 @@ extern "C" int vx_gemm_q4(const void* x, const void* codes, const void* affine, 
     if (K <= 0 || (group != 32 && group != 64 && group != 128) || K % group || ldx < K || ldo < N) return VX_ERR_SHAPE;
     if (codes1 && (!affine1 || bias || act < 0 || act > VX_ACT_LAST)) return VX_ERR_SHAPE;
     if (ldx & 7 || (((uintptr_t)x) | ((uintptr_t)codes) | ((uintptr_t)affine) | ((uintptr_t)codes1) | ((uintptr_t)affine1)) & 15) return VX_ERR_ALIGN;
+    if (M > Q4_MOST || N > Q4_MOST || K > Q4_MOST) return VX_ERR_LIMIT;
     if (!q4_few(M, N, K, codes1 != nullptr))
         return vx_gemm_q4_tc(x, codes, affine, codes1, affine1, bias, out, M, N, K, ldx, ldo, group, act, out_dtype, w_ready, error, stream);
     const Q4Pair w = {{(const unsigned*)codes, (const unsigned*)codes1}, {(const unsigned*)affine, (const unsigned*)affine1}};

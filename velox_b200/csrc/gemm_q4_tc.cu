@@ -33,6 +33,7 @@
 #define QT_ROOM (224 * 1024) // shared memory for stages
 #define QT_CODES 8192        // bytes of a stage: codes of 128 rows by 128 k
 #define QT_AFFINE 2048       // ... room for their scales and offsets (512, 1024, 2048 for groups of 128, 64, 32)
+#define QT_MOST_K (1 << 24)  // depth up to which a tile takes well under the second that its epilogue waits for (131,072 steps of up to 0.93 us)
 #define QT_ERR_PRODUCER 10
 #define QT_ERR_MMA 11
 #define QT_ERR_EPILOGUE 12
@@ -450,6 +451,7 @@ extern "C" int vx_gemm_q4_tc_shape(const void* x, const void* codes, const void*
                                    void* out, int M, int N, int K, int ldx, int ldo, int group, int act, int out_dtype, int w_ready, int n,
                                    int splits, int* error, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return VX_OK;
+    if (M > Q4_MOST || N > Q4_MOST || K > QT_MOST_K) return VX_ERR_LIMIT;
     const int mats = codes1 ? 2 : 1, blocks = (K + 63) / 64, steps = (blocks + 1) / 2;
     if (K <= 0 || !error || n < 16 || n > 256 / mats || (n & 15) || splits < 1 || splits > 8 || splits > steps) return VX_ERR_SHAPE;
     if ((group != 32 && group != 64 && group != 128) || K % group || ldx < K || ldo < N) return VX_ERR_SHAPE;
@@ -469,7 +471,6 @@ extern "C" int vx_gemm_q4_tc_shape(const void* x, const void* codes, const void*
     QtMaps maps;
     const long long wt = (N + 15) / 16, words = (long long)blocks * Q4_BLOCK_WORDS, pairs = (long long)blocks * 64 / group * 16;
     const int box = QT_K / group * 16;
-    if (words > 0xffffffffLL) return VX_ERR_LIMIT;
     if (!tc_make_map(&maps.x, x, M, K, ldx, n) || !qt_make_map(&maps.codes[0], codes, wt, words, 2 * Q4_BLOCK_WORDS) ||
         !qt_make_map(&maps.affine[0], affine, wt, pairs, box))
         return VX_ERR_DRIVER;
@@ -480,7 +481,7 @@ extern "C" int vx_gemm_q4_tc_shape(const void* x, const void* codes, const void*
     static int sm_counts[VX_MAX_DEVICES];
     const int sms = vx_sm_count(sm_counts);
     const long long tiles = (long long)((N + 127) / 128) * ((M + n - 1) / n);
-    if (tiles > 0x7fffff) return VX_ERR_LIMIT;
+    if (tiles > 0x7fffff || (tiles / sms + 1) * steps > 0x7fffffff) return VX_ERR_LIMIT;   // (a block counts its steps in 31 bits)
     const int teams = sh.splits > 1 ? (int)tiles : (int)(tiles < sms ? tiles : sms);
 #define QT_GO(G_, T_) qt_launch<G_, T_>(maps, bias, (T_*)out, M, N, blocks, ldo, act, group, w_ready, sh, bytes + 1024, teams, error, stream)
     if (out_dtype == VX_F32) return QT_GO(false, float);
@@ -551,6 +552,7 @@ extern "C" int vx_gemm_q4_tc(const void* x, const void* codes, const void* affin
                              cudaStream_t stream) {
     if (M <= 0 || N <= 0) return VX_OK;
     if (K <= 0) return VX_ERR_SHAPE;
+    if (M > Q4_MOST || N > Q4_MOST || K > QT_MOST_K) return VX_ERR_LIMIT;
     static int sm_counts[VX_MAX_DEVICES];
     const QtPlan p = qt_plan(M, N, K, codes1 != nullptr, vx_sm_count(sm_counts));
     return vx_gemm_q4_tc_shape(x, codes, affine, codes1, affine1, bias, out, M, N, K, ldx, ldo, group, act, out_dtype, w_ready, p.n, p.splits, error,

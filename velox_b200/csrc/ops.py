@@ -2095,7 +2095,7 @@ def _q4_product(what: str, a: torch.Tensor, w: Q4Matrix, up: Optional[Q4Matrix],
 def gemm_q4(a: torch.Tensor, w: Q4Matrix, bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
             w_ready: bool = False) -> torch.Tensor:
     """a [M, K] (bfloat16) times the matrix that `w` [N, K] stands for, transposed (+ float32 `bias` [N]); float32 sums, rounded once to
-    `out_dtype` (bfloat16 or float32).  `w_ready`: see `gemm_nt_simt`."""
+    `out_dtype` (bfloat16 or float32).  More than a few rows: a K of at most 2^24.  `w_ready`: see `gemm_nt_simt`."""
     if a.is_cuda:
         out = (_CALLS or _calls()).gemm_q4(a, w.parts, None, bias, 0, out_dtype or torch.bfloat16, w_ready, _error_address(a.device))
         if out is not None:

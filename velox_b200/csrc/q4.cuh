@@ -17,6 +17,9 @@
 
 #define Q4_BLOCK_WORDS 128   // 32-bit words of a block of 16 rows by 64 k
 
+// Sizes up to here can be rounded up to a tile's and stay within 31 bits.
+#define Q4_MOST 0x7fffff00
+
 // Both halves of a register: the scale, the offset.
 __device__ __forceinline__ unsigned q4_scale(unsigned affine) { return __byte_perm(affine, 0, 0x1010); }
 __device__ __forceinline__ unsigned q4_offset(unsigned affine) { return __byte_perm(affine, 0, 0x3232); }

@@ -190,6 +190,7 @@ static int q4_grid(int N, int units, dim3* grid) {
 extern "C" int vx_quantize_q4(const void* W, void* codes, void* affine, int N, int K, long long ldw, int group, int dtype, cudaStream_t stream) {
     if (N <= 0) return VX_OK;
     if (K <= 0 || (group != 32 && group != 64 && group != 128) || K % group || ldw < K) return VX_ERR_SHAPE;
+    if (N > Q4_MOST || K > Q4_MOST) return VX_ERR_LIMIT;
     if (dtype != VX_F32 && dtype != VX_BF16) return VX_ERR_DTYPE;
     if ((((uintptr_t)W) | ((uintptr_t)codes) | ((uintptr_t)affine)) & 15 || (ldw * (dtype == VX_F32 ? 4 : 2)) & 15) return VX_ERR_ALIGN;
     const int blocks = (K + 63) / 64, groups = blocks * 64 / group;
@@ -215,6 +216,7 @@ extern "C" int vx_quantize_q4(const void* W, void* codes, void* affine, int N, i
 extern "C" int vx_dequantize_q4(const void* codes, const void* affine, void* W, int N, int K, int group, cudaStream_t stream) {
     if (N <= 0) return VX_OK;
     if (K <= 0 || (group != 32 && group != 64 && group != 128) || K % group) return VX_ERR_SHAPE;
+    if (N > Q4_MOST || K > Q4_MOST) return VX_ERR_LIMIT;
     if ((((uintptr_t)W) | ((uintptr_t)codes) | ((uintptr_t)affine)) & 15) return VX_ERR_ALIGN;
     const int blocks = (K + 63) / 64, groups = blocks * 64 / group;
     dim3 grid;
