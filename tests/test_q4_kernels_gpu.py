@@ -384,3 +384,25 @@ def test_refusals():
             (lambda: ops.quantize_q4(x[:, 1:65], 64), "aligned"), (lambda: ops.quantize_q4(x.t(), 64), "contiguous")]:
         with pytest.raises(ops.KernelError, match=why):
             call()
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_groups_that_fill_the_range_of_float32(group):
+    """max - min just below float32's largest: w - b may overflow where b is the minimum rounded away, and the largest value's code is 15 all the same."""
+    n = 96
+    g = torch.Generator().manual_seed(group)
+    u = torch.rand(n, group, generator=g).numpy()
+    span = np.linspace(3.36e38, 3.4028e38, n)[:, None]
+    low = -span * np.linspace(0.5, 0.503, 7)[np.arange(n) % 7][:, None]
+    u[:, 1], u[:, group - 2] = 0, 1
+    w = (low + span * u).astype(np.float32)
+    w[0] = -1.709387e38
+    w[0, 5:] = np.float32(1.693113e38)
+    want = q4.quantise(w, group)
+    top = np.isfinite(want[1][:, 0])
+    with np.errstate(over="ignore"):
+        overflows = top & ~np.isfinite(w.max(1) - want[2][:, 0].astype(np.float32))
+    assert top[0] and overflows[0] and overflows.sum() >= 4 and (top & ~overflows).sum() >= 4
+    assert (want[0][np.arange(n), w.argmax(1)][top] == 15).all()
+    for got, x in zip(q4.unpack(ops.quantize_q4(torch.from_numpy(w).cuda(), group)), want):
+        assert np.array_equal(got, x, equal_nan=True)

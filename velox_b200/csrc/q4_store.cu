@@ -58,7 +58,9 @@ template <> struct Q4Row<bf16> {
 };
 
 // Eight codes of one word.  The quotient is a product with y = 1 / s and one correction by its exact remainder (Markstein's theorem: with y
-// rounded correctly that gives the quotient rounded correctly, so ties are ties), a division only where a remainder could underflow.
+// rounded correctly that gives the quotient rounded correctly, so ties are ties), a division only where a remainder could underflow, or where
+// float32 values are so large that w - b can overflow although max - min does not (b is a float32 minimum rounded, maybe away from the values; of
+// bfloat16 values it is the minimum itself): infinity divided by s is bounded by 15, its remainder would be NaN.
 // (Dividing always, 12288 x 4096 bfloat16 in groups of 64 took 78 us; dividing where the plain product was within 1e-5 of half way, as some value of
 // a word's 256 mostly was, 39.)  Rounding is the addition of 1.5 * 2^23: the code is the sum's low bits, and the sums, shifted, add up to the word
 // and a constant.  Of bfloat16 values only the scale's own rounding takes a quotient beyond 15, to 15.06: no bounds are needed.
@@ -66,7 +68,7 @@ template <typename T>
 __device__ __forceinline__ unsigned q4_codes(const Q4Row<T>& row, int first, float s, float b, float inverse) {
     constexpr unsigned MAGIC = 0x4b400000u;   // 1.5 * 2^23
     unsigned word = 0, sums = 0;
-    if (s >= 1e-30f) {
+    if (s >= 1e-30f && (sizeof(T) == 2 || s <= 1e37f)) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int at = 4 * (4 * (i & 1) + (i >> 1));
