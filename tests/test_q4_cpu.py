@@ -130,3 +130,21 @@ def test_the_command_line_names_the_settings():
     assert args.weight_bits is None and args.head_bits is None and args.weight_group == 64
     with pytest.raises(SystemExit):
         build_parser().parse_args(["generate", "--weight-bits", "8"])
+
+
+@pytest.mark.parametrize("rows", [2 ** 31 - 256, 2139095040, 2100000000, 2080374784, 2021195833])
+def test_rows_up_to_the_limit_find_a_tile(rows):
+    """The tile's choice counts within 31 bits for as many rows as the entry point takes: a refusal (two rounds of tiles too many), not the end of the
+    process.  In a process of its own, which a division by zero would end."""
+    import subprocess
+    import sys
+    code = """
+from velox_b200.csrc import ops
+A = 1 << 20
+for codes1 in (None, A):
+    print(ops.library().vx_gemm_q4(A, A, A, codes1, codes1, None, A, %d, 256, 64, 64, 256, 64, 0, 1, 0, A, None))
+""" % rows
+    from helpers import ROOT
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=ROOT)
+    assert out.returncode == 0, out.stderr
+    assert [int(v) for v in out.stdout.split()] == [LIMIT, LIMIT]

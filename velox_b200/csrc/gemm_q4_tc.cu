@@ -458,6 +458,10 @@ extern "C" int vx_gemm_q4_tc_shape(const void* x, const void* codes, const void*
     if (codes1 && (!affine1 || bias || act < 0 || act > VX_ACT_LAST)) return VX_ERR_SHAPE;
     if (out_dtype != VX_BF16 && (out_dtype != VX_F32 || codes1)) return VX_ERR_DTYPE;
     if (ldx & 7 || (((uintptr_t)x) | ((uintptr_t)codes) | ((uintptr_t)affine) | ((uintptr_t)codes1) | ((uintptr_t)affine1)) & 15) return VX_ERR_ALIGN;
+    static int sm_counts[VX_MAX_DEVICES];
+    const int sms = vx_sm_count(sm_counts);
+    const long long tiles = (long long)((N + 127) / 128) * ((M + n - 1) / n);
+    if (tiles > 0x7fffff || (tiles / sms + 1) * steps > 0x7fffffff) return VX_ERR_LIMIT;   // (a block counts its steps in 31 bits)
     QtShape sh;
     sh.n = n;
     sh.steps = (steps + splits - 1) / splits;
@@ -478,10 +482,6 @@ extern "C" int vx_gemm_q4_tc_shape(const void* x, const void* codes, const void*
     maps.affine[1] = maps.affine[0];
     if (codes1 && (!qt_make_map(&maps.codes[1], codes1, wt, words, 2 * Q4_BLOCK_WORDS) || !qt_make_map(&maps.affine[1], affine1, wt, pairs, box)))
         return VX_ERR_DRIVER;
-    static int sm_counts[VX_MAX_DEVICES];
-    const int sms = vx_sm_count(sm_counts);
-    const long long tiles = (long long)((N + 127) / 128) * ((M + n - 1) / n);
-    if (tiles > 0x7fffff || (tiles / sms + 1) * steps > 0x7fffffff) return VX_ERR_LIMIT;   // (a block counts its steps in 31 bits)
     const int teams = sh.splits > 1 ? (int)tiles : (int)(tiles < sms ? tiles : sms);
 #define QT_GO(G_, T_) qt_launch<G_, T_>(maps, bias, (T_*)out, M, N, blocks, ldo, act, group, w_ready, sh, bytes + 1024, teams, error, stream)
     if (out_dtype == VX_F32) return QT_GO(false, float);
@@ -530,7 +530,7 @@ static QtPlan qt_plan(int M, int N, int K, bool gated, int sms) {
     QtPlan best = {};
     double least = 0;
     for (int rows = most, last = 0; rows >= 16; rows -= 16) {
-        const int xt = (M + rows - 1) / rows, n = ((M + xt - 1) / xt + 15) & ~15;   // (as even as xt tiles can be)
+        const int xt = (M + rows - 1) / rows, n = ((M - 1) / xt + 16) & ~15;   // (as even as xt tiles can be)
         if (n == last) continue;
         last = n;
         const long long tiles = (long long)wtiles * ((M + n - 1) / n);
