@@ -148,3 +148,10 @@ for codes1 in (None, A):
     out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=ROOT)
     assert out.returncode == 0, out.stderr
     assert [int(v) for v in out.stdout.split()] == [LIMIT, LIMIT]
+
+
+def test_rows_up_to_which_a_matrix_is_streamed():
+    few = ops.library().vx_gemm_q4_few_rows
+    assert [few(n, k, g) for n, k, g in [(4096, 4096, 0), (4096, 4096, 1), (12288, 4096, 0), (64, 64, 1), (2 ** 31 - 256, 2 ** 31 - 256, 1)]] == [32, 16, 16, 32, 16]
+    m = ops.Q4Matrix(*tensors(), 20, 96, 32)
+    assert m.few_rows(False) == m.few_rows(True) == 32

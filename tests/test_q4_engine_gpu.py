@@ -139,3 +139,29 @@ def test_the_command_line(model_folders):
                           "4", "--weight-bits", "4", "--head-bits", "4", "--num-pages", "16", "--max-model-len", "64"], capture_output=True, text=True, timeout=300)
     assert out.returncode == 0, out.stderr
     assert len(json.loads(out.stdout.splitlines()[0])["tokens"]) == 4
+
+
+@pytest.mark.parametrize("requests,waiting", [(40, 9), (20, 0)])
+def test_replayed_decode_steps_of_many_requests(model_folders, requests, waiting):
+    """40 requests: all nine products of a captured decode step run on the tensor cores' kernel, and each replay says so; 20 requests stream these small
+    matrices, and no replay has anything to be checked."""
+    from velox_b200 import SamplingParams
+    from velox_b200.csrc import ops
+    cfg, w = P.load_model_folder(model_folders["tiny_c"])
+    e = engine(model_folders["tiny_c"], "tiny_c", max_running_requests=64, head_bits=4)
+    prompts = [random_tokens(cfg["vocab_size"], 2 + i % 5, 900 + i) for i in range(requests)]
+    ids = [e.add_request(p, SamplingParams(max_tokens=7)) for p in prompts]
+    e.step()
+    assert all(len(e.request(i).generated) == 1 for i in ids)
+    counts = []
+    while e.scheduler.has_work():
+        before = ops.bounded_wait_launches()
+        e.step()
+        counts.append(ops.bounded_wait_launches() - before)
+        assert not ops.bounded_wait_pending()
+    assert len(counts) == 6 and counts[1:] == [waiting] * 5   # (the first of them is recorded)
+    graphs = list(e.runner.graphs.graphs.values())
+    assert len(graphs) == 1 and graphs[0].graph is not None and graphs[0].bounded_wait_launches == waiting
+    plain = four_bits(w, "tiny_c", True)
+    for p, i in zip(prompts, ids):
+        check_greedy_path(cfg, plain, p, list(e.scheduler.finished[i].generated), "bfloat16")

@@ -406,3 +406,19 @@ def test_groups_that_fill_the_range_of_float32(group):
     assert (want[0][np.arange(n), w.argmax(1)][top] == 15).all()
     for got, x in zip(q4.unpack(ops.quantize_q4(torch.from_numpy(w).cuda(), group)), want):
         assert np.array_equal(got, x, equal_nan=True)
+
+
+@pytest.mark.parametrize("m,n,k,plain,gated", [(16, 9000, 4096, 0, 0), (17, 512, 512, 0, 0), (32, 4096, 4096, 0, 1), (32, 1000, 2048, 0, 0), (17, 9000, 4096, 1, 1),
+                                               (33, 64, 64, 1, 1)])
+def test_the_products_that_wait_are_counted(m, n, k, plain, gated):
+    """A launch is counted as one with bounded waits where the kernel that ran has them, through the call module and without it."""
+    w = ops.quantize_q4(torch.zeros(n, k, dtype=torch.bfloat16, device="cuda"), 64)
+    x, _ = rows_of(m, k, 1)
+    ways = {False: [lambda: ops.gemm_q4(x, w), lambda: ops._q4_product("gemm_q4", x, w, None, None, torch.bfloat16, 0, False)],
+            True: [lambda: ops.gated_q4(x, w, w), lambda: ops._q4_product("gated_q4", x, w, w, None, torch.bfloat16, 0, False)]}
+    for pair, calls in ways.items():
+        for call in calls:
+            before = ops.bounded_wait_launches()
+            call()
+            assert ops.bounded_wait_launches() - before == (gated if pair else plain)
+    ops.check_device_errors()

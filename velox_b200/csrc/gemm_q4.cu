@@ -283,7 +283,8 @@ static int q4_launch(const bf16* x, const Q4Pair& w, const float* bias, TO* out,
 // Rows up to which the kernel above is taken: 16, or 32 where the matrix is small.  us, this way and on tcgen05: 16 rows 4096 x 4096 5.9, 9.6; gated
 // 12288 x 4096 22.8, 24.8; gated 17408 x 5120 33.5, 31.1; 32 rows 2048 x 2048 3.7, 5.9; 4096 x 4096 8.7, 9.6; 6144 x 4096 12.3, 11.8; 7168 x 5120
 // 15.3, 14.0; gated 9728 x 2560 23.0, 16.8; 24 rows 6144 x 4096 11.3, 11.8; 4096 x 12288 18.9, 15.8.
-static bool q4_few(int M, int N, int K, bool gated) { return M <= 16 || (M <= 32 && (long long)N * K * (gated ? 2 : 1) <= 26000000LL); }
+// (The only place that knows: whoever counts kernels with bounded waits asks here.)
+extern "C" int vx_gemm_q4_few_rows(int N, int K, int gated) { return (long long)N * K * (gated ? 2 : 1) <= 26000000LL ? 32 : 16; }
 
 extern "C" int vx_gemm_q4_tc(const void* x, const void* codes, const void* affine, const void* codes1, const void* affine1, const float* bias,
                              void* out, int M, int N, int K, int ldx, int ldo, int group, int act, int out_dtype, int w_ready, int* error,
@@ -299,7 +300,7 @@ extern "C" int vx_gemm_q4(const void* x, const void* codes, const void* affine, 
     if (codes1 && (!affine1 || bias || act < 0 || act > VX_ACT_LAST)) return VX_ERR_SHAPE;
     if (ldx & 7 || (((uintptr_t)x) | ((uintptr_t)codes) | ((uintptr_t)affine) | ((uintptr_t)codes1) | ((uintptr_t)affine1)) & 15) return VX_ERR_ALIGN;
     if (M > Q4_MOST || N > Q4_MOST || K > Q4_MOST) return VX_ERR_LIMIT;
-    if (!q4_few(M, N, K, codes1 != nullptr))
+    if (M > vx_gemm_q4_few_rows(N, K, codes1 != nullptr))
         return vx_gemm_q4_tc(x, codes, affine, codes1, affine1, bias, out, M, N, K, ldx, ldo, group, act, out_dtype, w_ready, error, stream);
     const Q4Pair w = {{(const unsigned*)codes, (const unsigned*)codes1}, {(const unsigned*)affine, (const unsigned*)affine1}};
 #define Q4_ROWS(G, T, GR, NT) q4_launch<G, T, GR, NT>((const bf16*)x, w, bias, (T*)out, M, N, K, ldx, ldo, act, w_ready, stream)

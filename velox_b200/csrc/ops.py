@@ -197,6 +197,7 @@ def _declare(lib) -> None:
         "vx_quantize_q4": [P, P, P, I, I, c_longlong, I, I, P],
         "vx_dequantize_q4": [P, P, P, I, I, I, P],
         "vx_gemm_q4": [P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, P, P],
+        "vx_gemm_q4_few_rows": [I, I, I],
         "vx_gemm_q4_tc_shape": [P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, P, P],
     }
     lib.vx_set_pdl_mask.argtypes = [I]
@@ -1968,7 +1969,7 @@ def gemm_bf16(a: torch.Tensor, w: torch.Tensor, bias=None, out_dtype: Optional[t
 
 
 Q4_GROUPS = (32, 64, 128)   # neighbours along a row that share a scale and an offset
-Q4_FEW_ROWS = 16            # rows up to which the products stream the matrix through mma.sync; above they have bounded waits
+Q4_FEW_ROWS = 16            # rows up to which the products stream any matrix through mma.sync; above `Q4Matrix.few_rows` says
 
 
 class Q4Matrix:
@@ -1976,7 +1977,7 @@ class Q4Matrix:
     `group` neighbours of a row.  Element (n, k) stands for bfloat16(q s + b), its code q and its group's bfloat16 scale s and offset b.
     Made by `quantize_q4`, or from tensors of that layout: codes int32 [ceil(rows / 16), ceil(depth / 64), 4, 8, 2, 2], affine
     bfloat16 [ceil(rows / 16), groups, 8, 2, 2], both contiguous."""
-    __slots__ = ("codes", "affine", "rows", "depth", "group", "parts")
+    __slots__ = ("codes", "affine", "rows", "depth", "group", "parts", "_few")
 
     def __init__(self, codes: torch.Tensor, affine: torch.Tensor, rows: int, depth: int, group: int):
         tiles, blocks, groups = _q4_sizes(rows, depth, group)
@@ -1987,13 +1988,22 @@ class Q4Matrix:
         _need(codes.device == affine.device, "Q4Matrix: codes on %s, scales and offsets on %s" % (codes.device, affine.device))
         _need(codes.data_ptr() % 16 == 0 and affine.data_ptr() % 16 == 0, "Q4Matrix: 16-byte aligned tensors")
         self.codes, self.affine, self.rows, self.depth, self.group = self.parts = (codes, affine, int(rows), int(depth), int(group))
+        self._few = None
 
     @classmethod
     def _of(cls, codes, affine, rows, depth, group):
         """(Tensors that a kernel has just laid out.)"""
         m = cls.__new__(cls)
         m.codes, m.affine, m.rows, m.depth, m.group = m.parts = (codes, affine, rows, depth, group)
+        m._few = None
         return m
+
+    def few_rows(self, gated: bool) -> int:
+        """Rows of a product with this matrix (a gated one with it and its like) up to which it is streamed through mma.sync; with
+        more the product has bounded waits."""
+        if self._few is None:
+            self._few = tuple(library().vx_gemm_q4_few_rows(self.rows, self.depth, g) for g in (0, 1))
+        return self._few[gated]
 
     @property
     def shape(self) -> Tuple[int, int]:
@@ -2060,11 +2070,11 @@ def dequantize_q4(w: Q4Matrix) -> torch.Tensor:
     return out
 
 
-def _q4_called(out, what: str):
+def _q4_called(out, w: Q4Matrix, gated: bool, what: str):
     """What the call module gave for a product (not None), its launch counted."""
     global _BOUNDED_WAIT_LAUNCHES
     out = _called(out, what)
-    if len(out) > Q4_FEW_ROWS:
+    if len(out) > Q4_FEW_ROWS and len(out) > w.few_rows(gated):
         _BOUNDED_WAIT_LAUNCHES += 1
     return out
 
@@ -2087,7 +2097,7 @@ def _q4_product(what: str, a: torch.Tensor, w: Q4Matrix, up: Optional[Q4Matrix],
         return out
     _check(library().vx_gemm_q4(_ptr(a), _ptr(w.codes), _ptr(w.affine), _ptr(up.codes) if up else None, _ptr(up.affine) if up else None, _ptr(bias),
                                 _ptr(out), m, w.rows, k, lda, w.rows, w.group, act, dtype_code(out_dtype), 1 if w_ready else 0, _error_address(a.device), _stream()), what)
-    if m > Q4_FEW_ROWS:
+    if m > w.few_rows(up is not None):
         note_bounded_wait()
     return out
 
@@ -2099,7 +2109,7 @@ def gemm_q4(a: torch.Tensor, w: Q4Matrix, bias: Optional[torch.Tensor] = None, o
     if a.is_cuda:
         out = (_CALLS or _calls()).gemm_q4(a, w.parts, None, bias, 0, out_dtype or torch.bfloat16, w_ready, _error_address(a.device))
         if out is not None:
-            return _q4_called(out, "gemm_q4")
+            return _q4_called(out, w, False, "gemm_q4")
     return _q4_product("gemm_q4", a, w, None, bias, out_dtype or torch.bfloat16, 0, w_ready)
 
 
@@ -2109,7 +2119,7 @@ def gated_q4(a: torch.Tensor, gate: Q4Matrix, up: Q4Matrix, activation: str = "s
     if a.is_cuda and activation in ACTIVATIONS:
         out = (_CALLS or _calls()).gemm_q4(a, gate.parts, up.parts, None, ACTIVATIONS[activation], torch.bfloat16, w_ready, _error_address(a.device))
         if out is not None:
-            return _q4_called(out, "gated_q4")
+            return _q4_called(out, gate, True, "gated_q4")
     _need(activation in ACTIVATIONS, "gated_q4: unknown activation %r" % (activation,))
     _need(gate.shape == up.shape and gate.group == up.group and gate.device == up.device,
           "gated_q4: gate %s and up %s of one shape, group and device" % (gate.shape, up.shape))
