@@ -422,3 +422,14 @@ def test_the_products_that_wait_are_counted(m, n, k, plain, gated):
             call()
             assert ops.bounded_wait_launches() - before == (gated if pair else plain)
     ops.check_device_errors()
+
+
+@pytest.mark.parametrize("m,n,k,group", [(9, 2400, 4096, 32), (12, 15000, 160, 32), (16, 7000, 1056, 32), (24, 15001, 160, 32), (32, 40000, 96, 32), (12, 40003, 96, 32),
+                                         (10, 15000, 320, 64), (24, 15001, 384, 128)])
+def test_blocks_that_have_one_buffer_for_their_sums(m, n, k, group):
+    """9 to 32 rows, matrices of so many rows that a block forms several tiles: with small groups its sums are held once, and what one tile's epilogue
+    reads is not overwritten by the next tile."""
+    (w, w64), (up, u64) = made(n, k, group, 21), made(n, k, group, 22)
+    x, x64 = rows_of(m, k, 23)
+    q4.close(ops.gemm_q4(x, w, None, torch.float32), x64 @ w64.T, q4.sum_bound(x64, w64), torch.float32)
+    q4.close(ops.gated_q4(x, w, up, "silu"), *q4.gated(x64, w64, u64, "silu"), torch.bfloat16)

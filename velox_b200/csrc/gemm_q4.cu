@@ -50,9 +50,13 @@ template <int FORM, int GROUP, int BLOCKS> struct Q4Step {
     static constexpr int mats = FORM == Q4_ONE ? 1 : 2, codes = BLOCKS * 512, affine = BLOCKS * 64 * 64 / GROUP, bytes = codes + affine;
 };
 
-// The warps' sums of a tile, in shared memory: two buffers where they are small.
-template <int FORM, int NT, int WARPS> struct Q4Sums {
-    static constexpr int buffers = NT > 2 ? 1 : 2, bytes = buffers * (FORM == Q4_ONE ? 1 : 2) * WARPS * 16 * (8 * NT + 1) * 4;
+// A block's shared memory: the warps' rings, and their sums of a tile, in two buffers where these are small and leave room for PER_SM blocks
+// on an SM (which has 228 KB, of which each block takes 1 KB more than its own).
+template <int FORM, int GROUP, int NT, int WARPS, int BLOCKS, int DEPTH, int PER_SM> struct Q4Room {
+    static constexpr int mats = Q4Step<FORM, GROUP, BLOCKS>::mats, ring = WARPS * DEPTH * mats * Q4Step<FORM, GROUP, BLOCKS>::bytes,
+                         sums = mats * WARPS * 16 * (8 * NT + 1) * 4, share = 228 * 1024 / PER_SM - 1024,
+                         buffers = NT <= 2 && ring + 2 * sums <= share ? 2 : 1, bytes = ring + buffers * sums;
+    static constexpr bool fits = bytes <= share;
 };
 
 template <int FORM, typename TO, int GROUP, int NT, int WARPS, int BLOCKS, int DEPTH, int PER_SM>
@@ -64,7 +68,7 @@ gemm_q4_kernel(const bf16* __restrict__ x, const Q4Pair w, const float* __restri
     static_assert(BLOCKS * 64 % GROUP == 0, "a step holds whole groups");
     constexpr int MATS = Step::mats, SLOT = MATS * Step::bytes;
     extern __shared__ __align__(16) unsigned char q4_ring[];
-    constexpr int RED = Q4Sums<FORM, NT, WARPS>::buffers;
+    constexpr int RED = Q4Room<FORM, GROUP, NT, WARPS, BLOCKS, DEPTH, PER_SM>::buffers;
     typedef float Sums[MATS][WARPS][16][8 * NT + 1];
     Sums* red = reinterpret_cast<Sums*>(q4_ring + WARPS * DEPTH * SLOT);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
@@ -246,13 +250,13 @@ static int q4_sms() {
 template <int FORM, typename TO, int GROUP, int NT, int WARPS, int BLOCKS, int DEPTH, int PER_SM>
 static int q4_go(const bf16* x, const Q4Pair& w, const float* bias, TO* out, int M, int N, int K, int ldx, int ldo, int act, int w_ready,
                  cudaStream_t stream) {
-    typedef Q4Step<FORM, GROUP, BLOCKS> Step;
+    typedef Q4Room<FORM, GROUP, NT, WARPS, BLOCKS, DEPTH, PER_SM> Room;
+    static_assert(Room::fits, "a whole round of blocks is on the SMs at once");
     const int blocks = (K + 63) / 64, rows = FORM == Q4_TWO ? 32 : 16, units = (N + rows - 1) / rows, room = q4_sms() * PER_SM;
-    const size_t smem = (size_t)WARPS * DEPTH * Step::mats * Step::bytes + Q4Sums<FORM, NT, WARPS>::bytes;
     auto kernel = gemm_q4_kernel<FORM, TO, GROUP, NT, WARPS, BLOCKS, DEPTH, PER_SM>;
     static bool configured[VX_MAX_DEVICES];
-    if (int rc = vx_configure_smem(kernel, smem, configured)) return rc;
-    VX_LAUNCH_K(VX_K_GEMM, kernel, (unsigned)(units < room ? units : room), WARPS * 32, smem, stream, x, w, bias, out, M, N, K, ldx, ldo, act, blocks,
+    if (int rc = vx_configure_smem(kernel, Room::bytes, configured)) return rc;
+    VX_LAUNCH_K(VX_K_GEMM, kernel, (unsigned)(units < room ? units : room), WARPS * 32, Room::bytes, stream, x, w, bias, out, M, N, K, ldx, ldo, act, blocks,
                 units, w_ready);
     VX_LAUNCH_CHECK();
     return VX_OK;
@@ -268,15 +272,14 @@ static int q4_launch(const bf16* x, const Q4Pair& w, const float* bias, TO* out,
     // 5120 two tiles 8.3 (one 8.7); 4 rows 151936 x 2560 49.8 (eight warps 55.0, one tile 53.2).  Gated: 1 row 12288 x 4096 15.5 (four warps 16.9), 9728 x
     // 2560 10.0 (10.8), 8 rows 17408 x 5120 four warps 26.2 (eight 28.0).
 #define Q4_GO(F_, W_, P_) return q4_go<F_, TO, GROUP, NT, W_, 4, 2, P_>(x, w, bias, out, M, N, K, ldx, ldo, act, w_ready, stream)
-    if constexpr (GATED) {
-        if (tiles > 6 * sms) Q4_GO(Q4_GATED, 4, 4);
-        Q4_GO(Q4_GATED, 8, 2);
-    } else {
+    constexpr int BOTH = GATED ? Q4_GATED : Q4_TWO;
+    constexpr int FOUR = Q4Room<BOTH, GROUP, NT, 4, 4, 2, 4>::fits ? 4 : 3;   // (17 to 32 rows in groups of 32: three blocks fit an SM)
+    if (tiles > (GATED ? 6 : 16) * sms) Q4_GO(BOTH, 4, FOUR);
+    if constexpr (!GATED) {
         if (tiles <= 2 * sms) Q4_GO(Q4_ONE, 8, 2);
         if (tiles <= 3 * sms) Q4_GO(Q4_ONE, 8, 3);
-        if (tiles <= 16 * sms) Q4_GO(Q4_TWO, 8, 2);
-        Q4_GO(Q4_TWO, 4, 4);
     }
+    Q4_GO(BOTH, 8, 2);
 #undef Q4_GO
 }
 
