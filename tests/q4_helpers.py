@@ -53,6 +53,20 @@ def sum_bound(x, w):
     return steps * 2.0 ** -23 * (np.abs(x) @ np.abs(w).T)
 
 
+def run_bound(x, w):
+    """The same for deep products, where the bound above says little: a step's error is at most 2^-23 of the sum that it adds to and of its own terms'
+    absolute sum.  What a step adds to is the sum of a run of neighbouring blocks of 64 k and of part of a block (both kernels cut k so): no larger
+    than the range of the sums up to a block, and the largest block's absolute sum."""
+    m, n, blocks = x.shape[0], w.shape[0], -(-x.shape[1] // 64)
+    at, low, high, most = np.zeros((m, n)), np.zeros((m, n)), np.zeros((m, n)), np.zeros((m, n))
+    for i in range(blocks):
+        a, b = x[:, 64 * i:64 * i + 64], w[:, 64 * i:64 * i + 64]
+        at = at + a @ b.T
+        low, high = np.minimum(low, at), np.maximum(high, at)
+        most = np.maximum(most, np.abs(a) @ np.abs(b).T)
+    return 2.0 ** -23 * ((x.shape[1] / 8 + 32) * (high - low + most) + np.abs(x) @ np.abs(w).T)
+
+
 def act(z, name):
     if name == "silu":
         return z / (1 + np.exp(-z))
@@ -63,10 +77,10 @@ def act(z, name):
     return np.maximum(z, 0) ** (2 if name == "relu2" else 1)
 
 
-def gated(x, wg, wu, name):
+def gated(x, wg, wu, name, of_sums=sum_bound):
     """(act(x wg^T) * (x wu^T), a bound on the error of the float32 values behind the result's rounding)."""
     g, u = x @ wg.T, x @ wu.T
-    dg, du = sum_bound(x, wg), sum_bound(x, wu)
+    dg, du = of_sums(x, wg), of_sums(x, wu)
     a = act(g, name)
     slope = 1.13 if name != "relu2" else 2 * (np.abs(g) + dg)   # (the largest slope of silu and gelu is below 1.13)
     # the activation itself: a few roundings of terms up to |g| (1 + erf and the like cancel for negative g)

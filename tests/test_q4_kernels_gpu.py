@@ -433,3 +433,18 @@ def test_blocks_that_have_one_buffer_for_their_sums(m, n, k, group):
     x, x64 = rows_of(m, k, 23)
     q4.close(ops.gemm_q4(x, w, None, torch.float32), x64 @ w64.T, q4.sum_bound(x64, w64), torch.float32)
     q4.close(ops.gated_q4(x, w, up, "silu"), *q4.gated(x64, w64, u64, "silu"), torch.bfloat16)
+
+
+@pytest.mark.parametrize("m,n,k,group", [(1, 96, 12288, 64), (8, 200, 17408, 128), (16, 64, 18432, 32), (24, 100, 12288, 64), (40, 130, 12288, 64), (200, 256, 17408, 128),
+                                         (700, 40, 25600, 64)])
+def test_deep_products(m, n, k, group):
+    """As deep as the way down of a feed-forward and deeper, within a bound that a lost block of k, or sums held in fewer bits, would break."""
+    (w, w64), (up, u64) = made(n, k, group, 31), made(n, k, group, 32)
+    x, x64 = rows_of(m, k, 33)
+    bound = q4.run_bound(x64, w64)
+    want = x64 @ w64.T
+    assert np.median(bound) < 2e-3 * np.abs(want).mean()
+    q4.close(ops.gemm_q4(x, w, None, torch.float32), want, bound, torch.float32)
+    q4.close(ops.gemm_q4(x, w), want, bound, torch.bfloat16)
+    q4.close(ops.gated_q4(x, w, up, "silu"), *q4.gated(x64, w64, u64, "silu", q4.run_bound), torch.bfloat16)
+    ops.check_device_errors()

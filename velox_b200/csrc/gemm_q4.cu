@@ -8,7 +8,8 @@
 // fragments of four products, which it makes bfloat16 in registers.  (Through registers alone the loads share what the warp waits on with
 // those of x, and every block waited for memory.)  k is permuted the same way for x, of which a lane reads 32 neighbouring bytes of a
 // row, a code block ahead, through L1.  The warps' sums are added in shared memory in warp order: the same result on every run, and a row's
-// result does not depend on the rows beside it.
+// result does not depend on the rows beside it.  (A warp's sum is the tensor cores' float32, cut towards zero every 16 k: root mean square error of a
+// float32 result, relative, 2e-7 at 2,560 k, 1.1e-6 at 12,288.)
 //
 // What bounds it: instructions.  Eight weights take 15 (three shifts, four three-input logic operations, eight packed multiply-adds, two of
 // which a pipe takes every four cycles), and all of a code block 87 to 94 warp instructions with its loads, products and share of a tile's end, against
