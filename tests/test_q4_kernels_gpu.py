@@ -448,3 +448,54 @@ def test_deep_products(m, n, k, group):
     q4.close(ops.gemm_q4(x, w), want, bound, torch.bfloat16)
     q4.close(ops.gated_q4(x, w, up, "silu"), *q4.gated(x64, w64, u64, "silu", q4.run_bound), torch.bfloat16)
     ops.check_device_errors()
+
+
+def test_results_of_more_than_31_bits_of_elements():
+    """2,000 rows by 1.2 million columns: the last rows and columns are those of a small product."""
+    m, n, k, tail = 2000, 1200000, 64, 160
+    assert m * n > 2 ** 31
+    codes = torch.zeros(n // 16, 1, 4, 8, 2, 2, dtype=torch.int32, device="cuda")
+    affine = torch.zeros(n // 16, 1, 8, 2, 2, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(2)
+    codes[-tail // 16:] = torch.randint(-2 ** 31, 2 ** 31 - 1, codes[-tail // 16:].shape, dtype=torch.int32, device="cuda", generator=g)
+    affine[-tail // 16:] = (torch.rand(affine[-tail // 16:].shape, device="cuda", generator=g) * 0.01).to(torch.bfloat16)
+    big = ops.Q4Matrix(codes, affine, n, k, 64)
+    w64 = q4.matrix(*q4.unpack(ops.Q4Matrix(codes[-tail // 16:].clone(), affine[-tail // 16:].clone(), tail, k, 64)), 64)
+    x, x64 = rows_of(m, k, 4)
+    for out_dtype in (torch.bfloat16, torch.float32):
+        got = ops.gemm_q4(x, big, None, out_dtype)
+        q4.close(got[:, -tail:], x64 @ w64.T, q4.sum_bound(x64, w64), out_dtype)
+        assert not bool(got[:, :-tail].any())
+        del got
+    got = ops.gated_q4(x, big, big)
+    q4.close(got[:, -tail:], *q4.gated(x64, w64, w64, "silu"), torch.bfloat16)
+    assert not bool(got[:, :-tail].any())
+    ops.check_device_errors()
+
+
+@pytest.mark.parametrize("m", [8, 14, 40])
+def test_rows_that_lie_far_apart(m):
+    """Rows of x, and of a result inside a wider tensor, whose offsets pass 31 bits of elements."""
+    n, k, group = 200, 320, 64
+    far = (2 ** 31 // (m - 1) + 64) // 8 * 8
+    assert (m - 1) * far > 2 ** 31 and far < 2 ** 31
+    (w, w64), (up, u64) = made(n, k, group, 41), made(n, k, group, 42)
+    x, x64 = rows_of(m, k, 43)
+    apart = torch.zeros((m - 1) * far + k, dtype=torch.bfloat16, device="cuda").as_strided((m, k), (far, 1))
+    apart.copy_(x)
+    q4.close(ops.gemm_q4(apart, w, None, torch.float32), x64 @ w64.T, q4.sum_bound(x64, w64), torch.float32)
+    q4.close(ops.gated_q4(apart, w, up), *q4.gated(x64, w64, u64, "silu"), torch.bfloat16)
+    del apart
+    lib, error = ops.library(), ops._error_address(x.device)
+    wide = torch.zeros((m - 1) * far + n, dtype=torch.bfloat16, device="cuda")
+    for second in (None, up):
+        assert lib.vx_gemm_q4(x.data_ptr(), w.codes.data_ptr(), w.affine.data_ptr(), second and second.codes.data_ptr(), second and second.affine.data_ptr(), None,
+                              wide.data_ptr(), m, n, k, k, far, group, ops.ACTIVATIONS["silu"], 1, 0, error, ops._stream()) == 0
+        inner = wide.as_strided((m, n), (far, 1))
+        if second:
+            q4.close(inner, *q4.gated(x64, w64, u64, "silu"), torch.bfloat16)
+        else:
+            q4.close(inner, x64 @ w64.T, q4.sum_bound(x64, w64), torch.bfloat16)
+        inner.zero_()
+        assert not bool(wide.any())
+    ops.check_device_errors()
