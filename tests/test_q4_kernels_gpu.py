@@ -499,3 +499,25 @@ def test_rows_that_lie_far_apart(m):
         inner.zero_()
         assert not bool(wide.any())
     ops.check_device_errors()
+
+
+def test_beside_the_dense_product_on_another_stream():
+    """Both products take tensor memory in clusters of blocks (24 rows: tiles of 16, k in four runs; dense: k in runs, two blocks an SM).  Their blocks never
+    share an SM, so no cluster waits for the other's tensor memory."""
+    w, _ = made(2048, 16384, 64, 1)
+    x, _ = rows_of(24, 16384, 2)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    dense = torch.randn(2048, 4096, generator=g, device="cuda").to(torch.bfloat16)
+    y = torch.randn(24, 4096, generator=g, device="cuda").to(torch.bfloat16)
+    want, also = ops.gemm_q4(x, w), ops.gemm_turned(y, dense, w_ready=True)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(40):
+        with torch.cuda.stream(streams[0]):
+            got.append(ops.gemm_q4(x, w, w_ready=True))
+        with torch.cuda.stream(streams[1]):
+            got += [ops.gemm_turned(y, dense, w_ready=True) for _ in range(3)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(v, also if i % 4 else want) for i, v in enumerate(got))
+    ops.check_device_errors()

@@ -22,8 +22,9 @@
 // Every wait on an mbarrier is bounded; a block whose wait runs out records a code in the caller's error word and writes NaN, the other roles run
 // out of their own, all meet, free their tensor memory and return.
 //
-// Tensor memory is taken before the wait for the kernel before and before the next one is let in (gemm_turned.cu says why that is safe:
-// every kernel that takes some after it lets the next one in fills an SM's shared memory, and so do these blocks all but).
+// Tensor memory is taken before the wait for the kernel before and before the next one is let in (gemm_turned.cu says why that is safe).  A block
+// takes all of it, and so much shared memory that no other block that takes some fits beside it, whatever stream that one is on: two clusters
+// whose blocks waited for each other's tensor memory on two SMs would wait for good, as a cluster gives none back before its blocks have met.
 #include "q4.cuh"
 #include "tcgen05_pair.cuh"
 
@@ -35,6 +36,7 @@
 #define QT_PLACES_AT 256     // W's values in tensor memory: 256 columns behind the accumulators
 #define QT_MAX_STAGES 8
 #define QT_ROOM (224 * 1024) // shared memory for stages
+#define QT_LEAST (160 * 1024)   // ... at least: the smallest ring beside tensor memory, of a turned product with two blocks an SM, is 84 KB
 #define QT_CODES 8192        // bytes of a stage: codes of 128 rows by 128 k
 #define QT_AFFINE 2048       // ... room for their scales and offsets (512, 1024, 2048 for groups of 128, 64, 32)
 #define QT_MOST_K (1 << 24)  // depth up to which a tile takes well under the second that its epilogue waits for (131,072 steps of up to 0.93 us)
@@ -475,7 +477,8 @@ extern "C" int vx_gemm_q4_tc_shape(const void* x, const void* codes, const void*
     size_t bytes = (size_t)sh.stages * stage;
     const size_t sums = (size_t)mats * n * 512;
     if (sh.splits > 1 && bytes < sums) bytes = sums;
-    if (bytes < 120 * 1024) bytes = 120 * 1024;   // (one block an SM: the tensor memory is one block's)
+    static_assert(QT_LEAST + 84 * 1024 > 228 * 1024, "no block that takes tensor memory fits beside one of these");
+    if (bytes < QT_LEAST) bytes = QT_LEAST;
     QtMaps maps;
     const long long wt = (N + 15) / 16, words = (long long)blocks * Q4_BLOCK_WORDS, pairs = (long long)blocks * 64 / group * 16;
     const int box = QT_K / group * 16;
