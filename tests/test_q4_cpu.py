@@ -155,3 +155,10 @@ def test_rows_up_to_which_a_matrix_is_streamed():
     assert [few(n, k, g) for n, k, g in [(4096, 4096, 0), (4096, 4096, 1), (12288, 4096, 0), (64, 64, 1), (2 ** 31 - 256, 2 ** 31 - 256, 1)]] == [32, 16, 16, 32, 16]
     m = ops.Q4Matrix(*tensors(), 20, 96, 32)
     assert m.few_rows(False) == m.few_rows(True) == 32
+
+
+def test_a_tied_head_needs_nothing_but_its_table():
+    from velox_b200.parts import OutputHead
+    head, table = OutputHead("h.", 30, 40, tied=True), torch.zeros(30, 40)
+    head.tie(table)
+    assert head.weight is table and head.q4 is None

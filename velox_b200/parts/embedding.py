@@ -115,7 +115,8 @@ class OutputHead(Part):
         self._take(table)
 
     def _take(self, weight: torch.Tensor) -> None:
-        self.q4 = linear(weight, None, self.runtime.head_group, self.weight_name) if self.runtime.head_group else None
+        runtime = getattr(self, "runtime", None)   # (a tied head may be given its table without having been bound)
+        self.q4 = linear(weight, None, runtime.head_group, self.weight_name) if runtime is not None and runtime.head_group else None
         self.weight = weight if self.q4 is None else None
 
     def forward(self, rows: torch.Tensor) -> torch.Tensor:
