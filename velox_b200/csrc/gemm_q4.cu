@@ -11,10 +11,11 @@
 // result does not depend on the rows beside it.  (A warp's sum is the tensor cores' float32, cut towards zero every 16 k: root mean square error of a
 // float32 result, relative, 2e-7 at 2,560 k, 1.1e-6 at 12,288.)
 //
-// What bounds it: instructions.  Eight weights take 15 (three shifts, four three-input logic operations, eight packed multiply-adds, two of
-// which a pipe takes every four cycles), and all of a code block 87 to 94 warp instructions with its loads, products and share of a tile's end, against
-// some 90 cycles that its bytes take at the copy rate.  us, and of the copy rate of 6,549 GB/s: gated 12288 x 4096 1 row 14.9, 58 %; gated 17408 x 5120
-// 8 rows 25.4, 61 %; 151936 x 2560 4 rows to float32 48.6, 69 %; 4096 x 12288 1 row 9.1, 48 %.
+// What bounds it: no unit alone.  Under the profiler 55 to 59 % of the issue slots are used, 48 to 51 % of the pipe for shifts and logic, 37 to 43 %
+// of that for packed multiply-adds, and some 60 % of the copy rate.  A warp's chain of load, values and products is covered by 15 warps an SM only in part,
+// every tile reads x again through L1, and some SMs have a tile more than others.  Eight weights take 15 instructions, a code block 87 to 94 for a
+// warp.  us in a captured row of calls, and of the copy rate of 6,549 GB/s: gated 12288 x 4096 1 row 14.8, 58 %; gated 17408 x 5120 8 rows 25.3, 61 %;
+// 151936 x 2560 4 rows to float32 48.7, 69 %; 4096 x 12288 1 row 9.0, 48 %.
 #include "q4.cuh"
 
 __device__ __forceinline__ unsigned q4_smem(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
@@ -269,9 +270,9 @@ static int q4_launch(const bf16* x, const Q4Pair& w, const float* bias, TO* out,
     const int tiles = (N + 15) / 16, sms = q4_sms();
     // Eight warps a tile, two blocks an SM; three where that lets all tiles be worked on at once; two tiles at a time where there are more; and
     // four warps by four blocks where there are so many that a tile's end, which all of a block's warps wait for, counts more than a tile's length.
-    // us, this way and the next best: 1 row 4096 x 4096 4.1 (two tiles 4.1, three blocks 4.8); 6144 x 4096 5.2 (two blocks 6.8, two tiles 5.9); 8 rows 7168 x
-    // 5120 two tiles 8.3 (one 8.7); 4 rows 151936 x 2560 49.8 (eight warps 55.0, one tile 53.2).  Gated: 1 row 12288 x 4096 15.5 (four warps 16.9), 9728 x
-    // 2560 10.0 (10.8), 8 rows 17408 x 5120 four warps 26.2 (eight 28.0).
+    // us, this way and the others: 1 row 4096 x 4096 4.2 (two tiles 4.3, three blocks 4.9); 6144 x 4096 5.3 (two blocks 6.6, two tiles 5.8); 8 rows 7168 x
+    // 5120 two tiles 7.9 (one, three blocks 10.1); 4 rows 151936 x 2560 to float32 48.7 (eight warps 53.4, one tile 61.9).  Gated: 1 row 12288 x 4096 14.8
+    // (four warps 16.1), 9728 x 2560 9.8 (10.0), 8 rows 17408 x 5120 four warps 25.3 (eight 26.7).
 #define Q4_GO(F_, W_, P_) return q4_go<F_, TO, GROUP, NT, W_, 4, 2, P_>(x, w, bias, out, M, N, K, ldx, ldo, act, w_ready, stream)
     constexpr int BOTH = GATED ? Q4_GATED : Q4_TWO;
     constexpr int FOUR = Q4Room<BOTH, GROUP, NT, 4, 4, 2, 4>::fits ? 4 : 3;   // (17 to 32 rows in groups of 32: three blocks fit an SM)
@@ -284,9 +285,10 @@ static int q4_launch(const bf16* x, const Q4Pair& w, const float* bias, TO* out,
 #undef Q4_GO
 }
 
-// Rows up to which the kernel above is taken: 16, or 32 where the matrix is small.  us, this way and on tcgen05: 16 rows 4096 x 4096 5.9, 9.6; gated
-// 12288 x 4096 22.8, 24.8; gated 17408 x 5120 33.5, 31.1; 32 rows 2048 x 2048 3.7, 5.9; 4096 x 4096 8.7, 9.6; 6144 x 4096 12.3, 11.8; 7168 x 5120
-// 15.3, 14.0; gated 9728 x 2560 23.0, 16.8; 24 rows 6144 x 4096 11.3, 11.8; 4096 x 12288 18.9, 15.8.
+// Rows up to which the kernel above is taken: 16, or 32 where the matrix is small.  us, this way and on tcgen05: 16 rows 4096 x 4096 6.2, 8.9; 4096 x
+// 12288 13.4, 14.6; gated 12288 x 4096 21.3, 24.9; gated 17408 x 5120 31.4, 31.4; 151936 x 2560 to float32 66.6, 66.4; 32 rows 2048 x 2048 3.9, 7.0;
+// 4096 x 4096 8.8, 9.5; 7168 x 5120 15.4, 13.5; gated 9728 x 2560 23.0, 16.8; 24 rows 4096 x 12288 18.8, 15.2.  At the limit, 6144 x 4096, the two are level
+// at 24 rows (11.4, 11.4) and 32 rows lose (12.4, 11.5).
 // (The only place that knows: whoever counts kernels with bounded waits asks here.)
 extern "C" int vx_gemm_q4_few_rows(int N, int K, int gated) { return (long long)N * K * (gated ? 2 : 1) <= 26000000LL ? 32 : 16; }
 

@@ -87,7 +87,7 @@ __device__ __forceinline__ float qt_ld_cluster(unsigned addr) {
 __device__ __forceinline__ void qt_arrive(unsigned bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
 }
-// z / (1 + exp(-z)) by the hardware's 2^x and 1 / x (a few 2^-23 each; the result is rounded to bfloat16, 2^-9).
+// z / (1 + exp(-z)) by the hardware's 2^x and 1 / x (a few 2^-23 each; the result is rounded to bfloat16, 2^-8).
 __device__ __forceinline__ float qt_silu(float z) {
     float e, d;
     asm("ex2.approx.f32 %0, %1;\n" : "=f"(e) : "f"(z * -1.4426950408889634f));

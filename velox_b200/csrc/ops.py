@@ -1976,7 +1976,7 @@ class Q4Matrix:
     """A matrix [rows, depth] held in four bits: `codes` and `affine` (scales and offsets) as `csrc/q4.cuh` lays them out, groups of
     `group` neighbours of a row.  Element (n, k) stands for bfloat16(q s + b), its code q and its group's bfloat16 scale s and offset b.
     Made by `quantize_q4`, or from tensors of that layout: codes int32 [ceil(rows / 16), ceil(depth / 64), 4, 8, 2, 2], affine
-    bfloat16 [ceil(rows / 16), groups, 8, 2, 2], both contiguous."""
+    bfloat16 [ceil(rows / 16), groups, 8, 2, 2], both contiguous, with zeros for k beyond the depth."""
     __slots__ = ("codes", "affine", "rows", "depth", "group", "parts", "_few")
 
     def __init__(self, codes: torch.Tensor, affine: torch.Tensor, rows: int, depth: int, group: int):

@@ -3,7 +3,7 @@
 // A row's K is cut into groups of 32, 64 or 128 neighbours.  A group keeps a bfloat16 scale s and offset b, its elements a code q from 0
 // to 15, and an element is W = bfloat16(q s + b): q s + b is rounded once, so every kernel multiplies with the same matrix, whatever the
 // number of rows.  (A scale has 8 significant bits and a code 4, so W would need 12 and more to be exact.  The rounding moves W by at most
-// half a step, 2^-9 of it; the code has moved it by up to half a scale, some 2^-5 of a group's largest element.)
+// half a step, 2^-8 of it; the code has moved it by up to half a scale, a thirtieth of the group's range.)
 //
 // Codes: blocks of 16 rows by 64 k, 512 bytes, along K first: [N / 16][K / 64][t 4][r 8][half 2][word 2] of 32 bits; row 16 i + 8 half + r,
 // k = 64 c + 16 t + 8 word + 2 p + e in bits 4 (4 e + p).
@@ -28,8 +28,9 @@ __device__ __forceinline__ unsigned q4_offset(unsigned affine) { return __byte_p
 // SMALL (a scale from 2^-126 up to 2^-5, as trained matrices have): a code in the lower bits of an otherwise empty bfloat16 is q 2^-133, a
 // subnormal number, exactly; with `scale` 2^133 as large their product is q s, and the multiply-add rounds q s + b once.
 // Else: a code in the lower bits of 128.0 (0x4300) is 128 + q exactly; less 128 exactly q.  That takes four more instructions for eight codes,
-// 15 instead of 11, on a pipe that is as busy as the one for shifts and logic.  (2048 rows, gated 12288 x 4096 339 and 322 us.  The kernel for a
-// few rows takes the longer way alone: both of them in its loop cost more than the shorter one gains, 151936 x 2560 48.7 and 58.9 us.)
+// 15 instead of 11, on a pipe that is as busy as the one for shifts and logic.  (2048 rows, gated 12288 x 4096: 339 us this way, 322 with the shorter
+// one, on one box.  The kernel for a few rows takes the longer way alone: both of them in its loop cost more than the shorter one gains, 4 rows
+// 151936 x 2560 58.9 us instead of 48.7.)
 template <bool SMALL>
 __device__ __forceinline__ void q4_values(unsigned word, unsigned scale, unsigned offset, unsigned (&w)[4]) {
 #pragma unroll

@@ -7,8 +7,9 @@
 // A warp makes a block of 16 rows by 64 k (groups of 128: two): lane 4 r + t holds rows r and r + 8, 16 k of each of a block, as the layout has them,
 // so a row's 64 k are 128 or 256 neighbouring bytes read by four lanes, a group's extremes two or one exchanges away, and a block's 512 bytes
 // are written at once.
-// What bounds them: memory.  12288 x 4096, us and of the copy rate of 6,549 GB/s: from bfloat16 in groups of 64 28.5, 69 % (some nine instructions an
-// element besides); from float32 35.5, 99 %; back 22.2, 89 %.
+// What bounds them: from bfloat16 instructions (some nine an element), else memory.  12288 x 4096 in groups of 64, us of calls in a row and of the copy
+// rate of 6,549 GB/s: from bfloat16 28.2, 70 % (33.6, 59 %, where every result goes to memory not written before); from float32 38.4, 91 %
+// (41.2, 85 %); back 22.8, 87 %.
 #include "q4.cuh"
 
 // 16 neighbours of a row as they are stored: their extremes, whether all are finite, their values.
